@@ -276,6 +276,55 @@ int seedmi_pack_skinny_weights(const void* W, int ldw, int N, int K, void* out, 
 int seedmi_gemm_skinny_packed_bf16(int M, int N, int K, const void* A, int lda, const void* W_packed, const void* residual,
                                    int ldr, int epilogue, void* C, int ldc, int a_packed, int c_packed, void* stream);
 
+/* ---- KV cache by handle: 16-bit or 8-bit rows, grouped heads, one length per slot, a prefix that slots share --------------------- */
+#define SEEDMI_KV_16BIT 0          /* rows of head_dim 16-bit elements (what the LLaMA path's static caches hold)                  */
+#define SEEDMI_KV_MX8 1            /* rows of head_dim e4m3 bytes + one power-of-two scale byte per 32 of them (1.03 bytes a value) */
+/* Keys and values of `slots` conversations, `kv_heads` heads each: row r of head h of slot s starts at element
+ * ((s * slot_rows + h * head_rows) + r) * head_dim of k / v and, for MX8, at byte ((s * slot_rows + h * head_rows) + r) * head_dim / 32 of
+ * k_scale / v_scale.  Rows 0 .. rows - 1 of every (slot, head) belong to the caller's allocation; nothing outside them is touched.
+ * A contiguous [slots][kv_heads][rows][head_dim] cache has head_rows = rows and slot_rows = kv_heads * rows.  head_dim is 64 or 128.
+ * k and v are 16-byte aligned, k_scale and v_scale 4-byte aligned (NULL for 16BIT).
+ * MX8: a = the largest finite magnitude of a block of 32; e = the smallest integer >= -126 with a <= 448 * 2^e; scale byte = e + 127; an
+ * element x is stored as e4m3(x / 2^e), to nearest even (off by at most 2^-4 of x, or 2^-10 * 2^e for the smallest).  Infinities and NaN
+ * are stored as NaN and do not enter a; magnitudes above 1.875 * 2^127 (fp16 build: 1.875 * 2^15) are stored as that, so that every finite
+ * value reads back finite.  Scale bytes 1 .. 254 are valid.
+ * (A tag and a typedef of its own: the struct has no counterpart in the reference's call surface.) */
+struct seedmi_kv_cache {
+    void *k, *v;
+    void *k_scale, *v_scale;
+    long long slot_rows, head_rows;
+    int slots, rows, kv_heads, head_dim, format;
+};
+typedef struct seedmi_kv_cache seedmi_kv_cache_t;
+/* seedmi_rope_kv_append for a cache handle: the rows of slots 0 .. B - 1 behind what each holds.  qkv [B*T, (H + 2 * kv_heads) * head_dim]
+ * (q | k | v, row stride ldqkv); queries and keys are rotated as half(half(x cos) + half(rotate_half(x) sin)) (bf16: bit-identical to
+ * seedmi_rope_kv_append; the fp16 build of that one fuses a product into the sum), queries go to q_out [B*T, H * head_dim] (row stride ldq), keys and values into cache rows n_b .. n_b + T - 1, where n_b = past_lens_i32[b]
+ * (device int32 [B]) or past_len when that is NULL.  The position of row (b, t) is pos_ids_i64[b * T + t], or pos_base + n_b + t when that
+ * is NULL (pos_base = the length of a shared prefix in front), clamped to [0, max_pos).  A slot whose device-resident length is negative is
+ * idle: nothing is written to the cache for it; rows at or beyond cache->rows are not written.  The rows of different (slot, head) pairs
+ * must not overlap. */
+int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv, int ldqkv, const void* pos_ids_i64, int pos_base, const void* cos_t,
+                     const void* sin_t, int max_pos, void* q_out, int ldq, int B, int T, int H, int past_len, const void* past_lens_i32,
+                     void* stream);
+/* Rows start_b .. start_b + n - 1 of slots 0 .. B - 1 of an MX8 cache as 16-bit values, k_out / v_out [B][kv_heads][n][head_dim] (either may
+ * be NULL); start_b = starts_i32[b] (device int32 [B]) or start when that is NULL.  Rows outside 0 .. cache->rows - 1 read as zeros. */
+int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int B, int n, int start, const void* starts_i32, void* stream);
+/* Attention of T query rows per slot over the slot's cache rows, H query heads on kv_heads key heads (head h reads key head
+ * h / (H / kv_heads)): out = softmax(scale * q k^T) v.  q and out are [B*T, H * head_dim] (row strides ldq, ldo).  Slot b holds
+ * n_b = kv_lens_i32[b] rows (device int32 [B]; kv_len when that is NULL), the T queries are its last rows: with causal != 0 query t sees
+ * rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all visible) rows 0 .. n_b - 1.  n_b is clamped to
+ * [0, cache->rows].  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
+ * head_dim), in front of its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros.
+ * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the
+ * probabilities (unnormalised, 0 .. 1) are rounded to the 16-bit element for the product with the values.
+ * kv_max: the longest n_b expected (0: cache->rows); it decides how the keys are split over workgroups and never what is computed.
+ * workspace: seedmi_kv_attention_workspace_bytes() bytes (may be 0), 256-byte aligned; needs no initialisation and carries nothing from one
+ * call to the next; calls that may overlap need one each. */
+size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* cache, int B, int T, int H, int kv_max, int prefix_len);
+int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq, void* out,
+                        int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale, int causal,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- path level: SEED-2 tokenizer ------------------------------------------------------------------------------ */
 typedef struct {
     const void *ln1_w, *ln1_b;      /* blocks.N.norm1                                   */

@@ -72,6 +72,13 @@ class LlamaWeights(C.Structure):
                  ("cos_t", _vp), ("sin_t", _vp), ("lm_head_p", _vp), ("norm_folded", _i)])
 
 
+class KVCacheStruct(C.Structure):
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] + [("slot_rows", C.c_longlong), ("head_rows", C.c_longlong)] +
+                [(n, _i) for n in ("slots", "rows", "kv_heads", "head_dim", "format")])
+
+
+KV_16BIT, KV_MX8 = 0, 1
+
 # name -> (restype, argtypes); must list every symbol include/seedmi.h declares (tests check the export table)
 SIGNATURES = {
     "seedmi_version": (_i, []),
@@ -122,6 +129,11 @@ SIGNATURES = {
     "seedmi_tokenize_fj": (_i, [C.POINTER(TokenizerWeights), _vp, _i, _i, _vp, C.POINTER(TokenizerTaps), _vp,
                                 C.c_size_t, C.POINTER(ForkJoin), _vp]),
     "seedmi_sample_token_bf16": (_i, [_vp, _i, _i, _i, C.c_float, C.c_float, _vp, _vp, _i, _vp, _vp, _i, _i, _vp]),
+    "seedmi_kv_append": (_i, [C.POINTER(KVCacheStruct), _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "seedmi_kv_read": (_i, [C.POINTER(KVCacheStruct), _vp, _vp, _i, _i, _i, _vp, _vp]),
+    "seedmi_kv_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KVCacheStruct), _i, _i, _i, _i, _i]),
+    "seedmi_kv_attention": (_i, [C.POINTER(KVCacheStruct), C.POINTER(KVCacheStruct), _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _i,
+                                 C.c_float, _i, _vp, C.c_size_t, _vp]),
     "seedmi_preprocess_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i]),
     "seedmi_preprocess_image_u8": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, C.POINTER(C.c_float), C.POINTER(C.c_float),
                                         _vp, _i, _vp, _vp, C.c_size_t, _vp]),
