@@ -14,7 +14,8 @@ def build(force=False):
     src = os.path.join(HERE, "calib.hip")
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(HERE, "seedcal.h")))
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
-        subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-o", LIB, src])
+        subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                               "-shared", "-fPIC", "-o", LIB, src])
     return LIB
 
 
