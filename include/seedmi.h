@@ -313,7 +313,7 @@ int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int
  * h / (H / kv_heads)): out = softmax(scale * q k^T) v.  q and out are [B*T, H * head_dim] (row strides ldq, ldo).  Slot b holds
  * n_b = kv_lens_i32[b] rows (device int32 [B]; kv_len when that is NULL), the T queries are its last rows: with causal != 0 query t sees
  * rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all visible) rows 0 .. n_b - 1.  n_b is clamped to
- * [0, cache->rows].  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
+ * [0, cache->rows]; scale is finite and above 0.  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
  * head_dim), in front of its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros.
  * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the
  * probabilities (unnormalised, 0 .. 1) are rounded to the 16-bit element for the product with the values.

@@ -181,59 +181,395 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, bf16_t* __
 }
 
 // ------------------------------------------------------------------------------------------------ attention
+// Query rows that read the same keys form a GROUP: the T * (H / G) rows of a (slot, key head) over the slot's own rows, or all
+// B * T * (H / G) rows of a key head over the shared prefix.  Row r of a group is token row base + r / GH (GH = H / G), head g * GH + r % GH.
+//
+// With s_j = c q.k_j (c = scale * log2 e) a range of keys gives m = max s_j, l = sum 2^(s_j - m), o = sum 2^(s_j - m) v_j; ranges join by
+// M = max m, (l, o) = sum 2^(m - M) (l, o), and out = o / l.
 struct AttnArgs {
-    KvView c, p;                                         // the slots' cache, the shared prefix
+    KvView c;                                            // the slots' cache, or the prefix as a cache of one slot
     const bf16_t* q;
-    bf16_t* out;
-    int ldq, ldo, B, T, H, kv_len, prefix_len, causal;
+    bf16_t* out;                                         // direct output (one part only), else NULL
+    float* o_part;                                       // [parts][B*T*H][HD] sums of a part
+    float2* ml_part;                                     // [parts][B*T*H] (m, l); l == 0: the part holds nothing for the row
     const int* kv_lens;
-    float scale;
+    int ldq, ldo, T, H, GH, kv_len, causal;
+    int groups, group_rows, row_blocks;                  // groups = slots * G of this pass, rows of a group, blocks of 16 MT rows
+    int shared;                                          // 1: the groups are those of the prefix (kv_len rows, all visible)
+    int splits, part0;                                   // key ranges of this pass and the first one's part index
+    long long rows;                                      // B * T * H
+    float c2;
 };
 
-// One wave = one query row: lane = HD / 64 values of the row, keys one after the other.
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+constexpr int KT = 32;                                   // keys of a tile
+constexpr int MIN_TILES = 4;                             // of a split: one tile per wave
+
+// maximum / sum over the four 16-lane rows of a wave (the lanes of one query): VALU row swaps, no LDS
+SEEDMI_DEVINL float rows_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+SEEDMI_DEVINL float rows_sum(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+SEEDMI_DEVINL float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// not finite: exponent field all ones, in both halves of a word of 16-bit elements
+SEEDMI_DEVINL uint32_t exp_mask16() {
+#ifdef SEEDMI_F16
+    return 0x7c00u;
+#else
+    return 0x7f80u;
+#endif
+}
+SEEDMI_DEVINL bool bad16(uint32_t h) { return (h & exp_mask16()) == exp_mask16(); }
+
+// A tile of 32 keys and values as a wave holds it between the load and its use.
+//   K (the MFMA's A operand, rows = keys): lane (li, g) holds its part of rows 16 kt + li.  16-bit rows: k-step ks = values 32 ks + 8 g ..;
+//     8-bit rows: 16 bytes at 64 j + 16 g = k-steps 2 j and 2 j + 1 (the contraction may run in any order that Q's fragments share).
+//   V: whole rows, lanes side by side.
 template <int HD, bool MX>
-__global__ __launch_bounds__(256) void kv_attention_rows_kernel(const AttnArgs a) {
-    constexpr int VPL = HD / 64;
-    const int lane = threadIdx.x & 63;
-    const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (long long)a.B * a.T * a.H) return;
-    const int h = (int)(r % a.H);
-    const int row = (int)(r / a.H);
-    const int b = row / a.T, t = row - b * a.T;
-    const int g = h / (a.H / a.c.G);
-    const int len = max(0, min(a.kv_lens ? a.kv_lens[b] : a.kv_len, a.c.rows));
-    const int seen = a.causal ? max(0, len - a.T + t + 1) : len;
-    float q[VPL], o[VPL], m = -INFINITY, l = 0.f;
+struct Tile {
+    static constexpr int KL = MX ? HD / 64 : HD / 32;    // 16-byte loads of a key row per lane
+    static constexpr int VL = MX ? HD / 32 : HD / 16;    // 16-byte loads of the value tile per lane
+    uint4 k[2][KL], v[VL];
+    uint32_t ks[2], vs[VL];
+};
+
+template <int HD, bool MX>
+SEEDMI_DEVINL void load_k(Tile<HD, MX>& t, const char* kb, const uint8_t* ksb, int key0, int last, int lane) {
+    constexpr int RB = MX ? HD : 2 * HD;                 // bytes of a row
+    const int li = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-        q[v] = bf2f(a.q[(size_t)row * a.ldq + h * HD + lane * VPL + v]) * a.scale;
-        o[v] = 0.f;
+    for (int kt = 0; kt < 2; ++kt) {
+        const long long row = min(key0 + 16 * kt + li, last);
+#pragma unroll
+        for (int j = 0; j < Tile<HD, MX>::KL; ++j) t.k[kt][j] = *(const uint4*)(kb + row * RB + 64 * j + 16 * g);
+        if (MX) t.ks[kt] = HD == 128 ? *(const uint32_t*)(ksb + row * 4) : (uint32_t)*(const uint16_t*)(ksb + row * 2);
     }
-    auto val = [&](const char* base, const uint8_t* sc, long long crow, int v) -> float {
-        const int d = lane * VPL + v;
-        if (!MX) return bf2f(((const bf16_t*)base)[crow * HD + d]);
-        const uint32_t w = mx_unpack2<false>((uint32_t)(uint8_t)base[crow * HD + d], mx_scale_f(sc[crow * (HD / 32) + d / 32]));
-        return lo_bf(w);
-    };
-    auto walk = [&](const KvView& c, long long first, int n) {
-        for (int j = 0; j < n; ++j) {
-            float s = 0.f;
+}
+template <int HD, bool MX>
+SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const char* vb, const uint8_t* vsb, int key0, int last, int lane) {
+    constexpr int RB = MX ? HD : 2 * HD;
+    constexpr int LPR = RB / 16;                         // lanes of a row
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) s += q[v] * val(c.k, c.ks, first + j, v);
-            s = wave_sum(s);
-            const float mn = fmaxf(m, s);
-            const float f = __expf(m - mn), p = __expf(s - mn);
-            l = l * f + p;
-            m = mn;
+    for (int j = 0; j < Tile<HD, MX>::VL; ++j) {
+        const long long row = min(key0 + j * (64 / LPR) + lane / LPR, last);
+        t.v[j] = *(const uint4*)(vb + row * RB + 16 * (lane % LPR));
+        if (MX) t.vs[j] = vsb[row * (HD / 32) + (lane % LPR) / 2];
+    }
+}
+
+// position of 16-byte chunk c of value row `row` in the LDS image: chunks are XOR-ed with the row, so that both the row-wise writes and the
+// transposing reads (4 rows x 32 bytes per 16 lanes) spread over the banks
+template <int HD>
+SEEDMI_DEVINL int v_chunk(int row, int c) { return row * (2 * HD) + ((c ^ (row & (HD / 8 - 1))) << 4); }
+
+// The value tile into the LDS image.  TAIL: rows from `rows` on become zeros; returns whether this lane saw a value that is not finite.
+template <int HD, bool MX, bool TAIL>
+SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int rows, int lane) {
+    constexpr int LPR = (MX ? HD : 2 * HD) / 16;
+    bool bad = false;
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) o[v] = o[v] * f + p * val(c.v, c.vs, first + j, v);
+    for (int j = 0; j < Tile<HD, MX>::VL; ++j) {
+        const int row = j * (64 / LPR) + lane / LPR, l = lane % LPR;
+        uint4 w = t.v[j];
+        if (TAIL && row >= rows) w = make_uint4(0, 0, 0, 0);
+        const uint32_t src[4] = {w.x, w.y, w.z, w.w};
+        if (MX) {
+            const float s = mx_scale_f(t.vs[j]);
+            uint32_t o[8];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                o[2 * d] = mx_unpack2<false>(src[d], s);
+                o[2 * d + 1] = mx_unpack2<true>(src[d], s);
+                if (TAIL) bad |= bad16(o[2 * d] & 0xffffu) | bad16(o[2 * d] >> 16) | bad16(o[2 * d + 1] & 0xffffu) | bad16(o[2 * d + 1] >> 16);
+            }
+            *(uint4*)(lds + v_chunk<HD>(row, 2 * l)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *(uint4*)(lds + v_chunk<HD>(row, 2 * l + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        } else {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                if (TAIL) bad |= bad16(src[d] & 0xffffu) | bad16(src[d] >> 16);
+            *(uint4*)(lds + v_chunk<HD>(row, l)) = w;
         }
-    };
-    if (a.prefix_len) walk(a.p, (long long)g * a.p.head_rows, a.prefix_len);
-    walk(a.c, (long long)b * a.c.slot_rows + (long long)g * a.c.head_rows, seen);
+    }
+    return bad;
+}
+
+// V^T fragment of channels 16 n .. + 15 from the LDS image: lane li = channel, keys 16 (j >> 2) + 4 g + (j & 3)
+template <int HD>
+SEEDMI_DEVINL bf16x8 v_frag(const char* lds, int n, int lane) {
+    const int li = lane & 15, g = lane >> 4;
+    const int row = 4 * g + (li >> 2), c = 2 * n + ((li & 3) >> 1), b8 = (li & 1) << 3;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_chunk<HD>(row, c) + b8));
+    const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_chunk<HD>(row + 16, c) + b8));
+    const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, z);
+    return __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y));
+}
+
+constexpr float LOWEST = -3.4028234e38f;
+SEEDMI_DEVINL void lds_fence() { asm volatile("" ::: "memory"); }        // (a wave's own LDS accesses are executed in order)
+
+// ---- few query rows per group (decode, drafted tokens, a shared prefix): bound by the bytes of the cache.
+// Workgroup = (group, block of 16 MT rows, key range); its 4 waves take the range's tiles in turn, each with a running softmax of its own,
+// and join at the end.  S^T = K Q^T (keys are the MFMA's rows: K fragments come straight from memory, one tile ahead in registers), so a
+// lane's scores are keys 4 g + r of its query li, which is the layout the P^T operand of O^T = V^T P^T needs: P never leaves registers.
+// V is transposed through 8 KiB of LDS that the wave has to itself (no barrier in the loop).
+template <int HD, bool MX, int MT>
+__global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void kv_attention_few_kernel(const AttnArgs a) {
+    constexpr int NT = HD / 16, KS = HD / 32;
+    constexpr int VBYTES = KT * HD * 2;
+    __shared__ __attribute__((aligned(16))) char sm[4 * (VBYTES > 16 * HD * 4 ? VBYTES : 16 * HD * 4)];
+    __shared__ float2 sml[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // eight items (XCDs) side by side, the row blocks of an item behind each other on its XCD
+    const unsigned items = (unsigned)a.groups * a.splits;
+    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    const unsigned item = blk * 8 + in % 8;
+    const int rb = in / 8;
+    if (item >= items) return;
+    const int split = item / a.groups, group = item % a.groups;
+    const int G = a.c.G, slot = group / G, kvh = group % G;
+    const int base = a.shared ? 0 : slot * a.T;          // first token row of the group
+    const int r0 = rb * 16 * MT, r_end = min(a.group_rows, r0 + 16 * MT);
+
+    int len = a.kv_len;
+    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
+    len = max(0, min(len, a.c.rows));
+    const bool causal = a.causal && !a.shared;
+    // rows of keys that a query row sees: all, or up to its own
+    const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
+    const int n_min = causal ? max(0, min(len, len - a.T + r0 / a.GH + 1)) : len;
+    const int tiles = (n_max + KT - 1) / KT;
+    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int t_begin = split * per, t_end = min(tiles, t_begin + per);
+
+    bf16x8 qf[MT][KS];
+    int seen[MT];
+    float m[MT], l[MT];
+    f32x4 o[MT][NT];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v)
-        a.out[(size_t)row * a.ldo + h * HD + lane * VPL + v] = f2bf(l == 0.f ? 0.f : o[v] / l);
+    for (int u = 0; u < MT; ++u) {
+        const int r = r0 + 16 * u + li;
+        const bool on = r < r_end;
+        seen[u] = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
+        const bf16_t* qp = a.q + (size_t)(base + (on ? r / a.GH : 0)) * a.ldq + (kvh * a.GH + (on ? r % a.GH : 0)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = MX ? 64 * (ks >> 1) + 16 * g4 + 8 * (ks & 1) : 32 * ks + 8 * g4;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (on) v = *(const uint4*)(qp + d);
+            qf[u][ks] = __builtin_bit_cast(bf16x8, v);
+        }
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    constexpr int RB = MX ? HD : 2 * HD;
+    const char* kb = a.c.k + row0 * RB;
+    const char* vb = a.c.v + row0 * RB;
+    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    char* lds = sm + wave * VBYTES;
+
+    const int last = n_max - 1;
+    Tile<HD, MX> t;
+    if (t_begin + wave < t_end) {
+        load_v(t, vb, vsb, (t_begin + wave) * KT, last, lane);
+        load_k(t, kb, ksb, (t_begin + wave) * KT, last, lane);
+    }
+#pragma unroll 1
+    for (int tile = t_begin + wave; tile < t_end; tile += 4) {
+        const int key0 = tile * KT, next0 = (tile + 4 < t_end ? tile + 4 : tile) * KT;
+        const bool partial = key0 + KT > n_min;          // (wave-uniform) some row of the block does not see all of the tile
+        bool mixed = false;
+        lds_fence();
+        if (!partial) stage_v<HD, MX, false>(t, lds, KT, lane);
+        else mixed = __any(stage_v<HD, MX, true>(t, lds, n_max - key0, lane));
+        lds_fence();
+        load_v(t, vb, vsb, next0, last, lane);           // the wave's next tile (its last one again at the end: no branch in the loop)
+        f32x4 s[MT][2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            bf16x8 kf[KS];
+#pragma unroll
+            for (int j = 0; j < Tile<HD, MX>::KL; ++j) {
+                const uint4 w = t.k[kt][j];
+                if (MX) {
+                    const float sc = mx_scale_f((t.ks[kt] >> (16 * j + 8 * (g4 >> 1))) & 255u);
+                    kf[2 * j] = __builtin_bit_cast(bf16x8, make_uint4(mx_unpack2<false>(w.x, sc), mx_unpack2<true>(w.x, sc), mx_unpack2<false>(w.y, sc), mx_unpack2<true>(w.y, sc)));
+                    kf[2 * j + 1] = __builtin_bit_cast(bf16x8, make_uint4(mx_unpack2<false>(w.z, sc), mx_unpack2<true>(w.z, sc), mx_unpack2<false>(w.w, sc), mx_unpack2<true>(w.w, sc)));
+                } else {
+                    kf[j] = __builtin_bit_cast(bf16x8, w);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s[u][kt] = seedmi_mfma_16x16x32(kf[ks], qf[u][ks], s[u][kt]);
+            }
+        }
+        load_k(t, kb, ksb, next0, last, lane);
+        bf16x8 pf[MT];
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+            if (partial) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (key0 + 16 * kt + 4 * g4 + r >= seen[u]) s[u][kt][r] = -INFINITY;
+            }
+            float tm = fmaxf(fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][0][2], s[u][0][3])),
+                             fmaxf(fmaxf(s[u][1][0], s[u][1][1]), fmaxf(s[u][1][2], s[u][1][3])));
+            tm = rows_max(tm) * a.c2;
+            const float mn = fmaxf(m[u], tm);
+            if (__any(mn > m[u])) {                      // a new maximum: what is summed so far is scaled down
+                const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
+                l[u] *= f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
+                m[u] = mn;
+            }
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            float p[2][4];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
+                    l[u] += p[kt][r];
+                }
+            pf[u] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0][0], p[0][1]), pack2bf(p[0][2], p[0][3]), pack2bf(p[1][0], p[1][1]), pack2bf(p[1][2], p[1][3])));
+        }
+        if (mixed) {
+            // Values that are not finite in a tile that some rows do not see whole: 0 * inf must not reach a row that does not see the key.
+            // They are added here to the rows that do, and taken out of the image.
+            lds_fence();
+#pragma unroll 1
+            for (int j = 0; j < KT; ++j) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 w = *(const uint2*)(lds + v_chunk<HD>(j, 2 * n + (g4 >> 1)) + 8 * (g4 & 1));
+                    const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int u = 0; u < MT; ++u)
+                            if (bad16(h[r]) && key0 + j < seen[u]) o[u][n][r] += bf2f((bf16_t)h[r]);
+                }
+            }
+            lds_fence();
+#pragma unroll 1
+            for (int i = 16 * lane; i < VBYTES; i += 1024) {
+                uint32_t* w = (uint32_t*)(lds + i);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t x = w[d], lo = x & 0xffffu, hi = x >> 16;
+                    w[d] = (bad16(lo) ? 0u : lo) | ((bad16(hi) ? 0u : hi) << 16);
+                }
+            }
+            lds_fence();
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const bf16x8 vf = v_frag<HD>(lds, n, lane);
+#pragma unroll
+            for (int u = 0; u < MT; ++u) o[u][n] = seedmi_mfma_16x16x32(vf, pf[u], o[u][n]);
+        }
+    }
+
+    // the four waves' (m, l, o) joined, one block of 16 rows at a time; thread = (row, HD / 16 channels)
+    float* so = (float*)sm;
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const float lsum = rows_sum(l[u]);
+        __syncthreads();
+        if (g4 == 0) sml[wave][li] = make_float2(m[u], lsum);
+        __syncthreads();
+        float M = LOWEST;                                // (finite: a sum that is NaN stays NaN, one that is 0 is left out)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w][li].x);
+        const float f = exp2_hw(fmaxf(m[u], LOWEST) - M);
+        // channel quads 4 (4 n + g) of row li, XOR-ed with the row
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x4 v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = lsum == 0.f ? 0.f : o[u][n][r] * f;
+            *(f32x4*)(so + (wave * 16 + li) * HD + (((4 * n + g4) ^ li) << 2)) = v;
+        }
+        __syncthreads();
+        const int row = tid >> 4, part = tid & 15;
+        const int r = r0 + 16 * u + row;
+        float L = 0.f, Mr = LOWEST;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) Mr = fmaxf(Mr, sml[w][row].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) L += sml[w][row].y * exp2_hw(fmaxf(sml[w][row].x, LOWEST) - Mr);
+        if (r < r_end) {
+            constexpr int Q = HD / 64;                   // quads of a thread
+            const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const int quad = part * Q + i;
+                f32x4 v = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const f32x4 x = *(const f32x4*)(so + (w * 16 + row) * HD + ((quad ^ row) << 2));
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) v[d] += x[d];
+                }
+                if (a.out) {
+                    const float inv = L == 0.f ? 0.f : 1.f / L;
+                    *(uint2*)(a.out + (size_t)token * a.ldo + head * HD + 4 * quad) = make_uint2(pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv));
+                } else {
+                    const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
+                    if (L != 0.f) *(f32x4*)(a.o_part + at * HD + 4 * quad) = v;
+                    if (part == 0 && i == 0) a.ml_part[at] = make_float2(Mr, L);
+                }
+            }
+        }
+    }
+}
+
+// The parts of every row joined: HD / 4 lanes per row.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml, long long rows,
+                                                                int parts, int H, bf16_t* __restrict__ out, int ldo) {
+    constexpr int LPR = HD / 4;
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
+    if (row >= rows) return;
+    const int d = 4 * (threadIdx.x % LPR);
+    float M = LOWEST;
+    for (int p = 0; p < parts; ++p) M = fmaxf(M, ml[p * rows + row].x);
+    float L = 0.f;
+    f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p) {
+        const float2 x = ml[p * rows + row];
+        if (x.y == 0.f) continue;                        // (a NaN sum is not skipped)
+        const float f = exp2_hw(x.x - M);
+        L += x.y * f;
+        const f32x4 v = *(const f32x4*)(o_part + (p * rows + row) * HD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += v[i] * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int token = (int)(row / H), head = (int)(row % H);
+    *(uint2*)(out + (size_t)token * ldo + head * HD + d) = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -340,24 +676,87 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
     return seedmi_check_launch("kv_read");
 }
 
-extern "C" size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* cache, int B, int T, int H, int kv_max, int prefix_len) {
-    (void)cache; (void)B; (void)T; (void)H; (void)kv_max; (void)prefix_len;
+// How a call is cut: a pass over the slots' own rows and, with a prefix, one over the prefix; row blocks and key ranges of each.
+struct KvPass { int groups, group_rows, mt, row_blocks, splits; };
+struct KvPlan { KvPass own, pre; int parts; long long rows; size_t bytes; };
+
+static KvPass plan_pass(int groups, long long rows, long long keys) {
+    KvPass p = {};
+    p.groups = groups;
+    p.group_rows = (int)rows;
+    p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    p.row_blocks = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
+    const long long tiles = (keys + KT - 1) / KT, base = (long long)groups * p.row_blocks;
+    long long s = (1024 + base - 1) / base;
+    if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
+    p.splits = (int)(s < 1 ? 1 : s);
+    return p;
+}
+
+// 0: fits; -1: not a shape the kernels take (the callers have checked pointers)
+static int make_plan(const seedmi_kv_cache_t* c, int B, int T, int H, int kv_max, int prefix_len, KvPlan* pl) {
+    if (!c || c->slots <= 0 || c->rows <= 0 || c->kv_heads <= 0 || B <= 0 || B > c->slots || T <= 0 || H <= 0 || H % c->kv_heads || kv_max < 0 ||
+        prefix_len < 0)
+        return -1;
+    pl->rows = (long long)B * T * H;
+    if (pl->rows > INT_MAX) return -1;
+    const int GH = H / c->kv_heads;
+    const long long keys = kv_max == 0 || kv_max > c->rows ? c->rows : kv_max;
+    if ((long long)B * c->kv_heads > INT_MAX / 64) return -1;
+    pl->own = plan_pass(B * c->kv_heads, (long long)T * GH, keys);
+    pl->pre = prefix_len ? plan_pass(c->kv_heads, (long long)B * T * GH, prefix_len) : KvPass{};
+    pl->parts = pl->own.splits + pl->pre.splits;
+    pl->bytes = pl->parts == 1 ? 0 : (((size_t)pl->parts * pl->rows * 8 + 255) & ~(size_t)255) + (size_t)pl->parts * pl->rows * c->head_dim * 4;
     return 0;
+}
+
+extern "C" size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* cache, int B, int T, int H, int kv_max, int prefix_len) {
+    KvPlan pl;
+    return make_plan(cache, B, T, H, kv_max, prefix_len, &pl) ? 0 : pl.bytes;
+}
+
+template <int HD, bool MX>
+static void launch_pass(const AttnArgs& a, const KvPass& p, hipStream_t s) {
+    const unsigned items = (unsigned)p.groups * p.splits;
+    const dim3 grid((items + 7) / 8 * 8 * p.row_blocks);
+    switch (p.mt) {
+        case 1: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 4>), grid, dim3(256), 0, s, a); break;
+    }
+}
+
+template <int HD, bool MX>
+static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, const KvPlan& pl, int prefix_len, bf16_t* out, hipStream_t s) {
+    a.out = pl.parts == 1 ? out : nullptr;
+    auto pass = [&](const KvView& v, const KvPass& p, int shared, int part0) {
+        AttnArgs x = a;
+        x.c = v;
+        x.groups = p.groups; x.group_rows = p.group_rows; x.row_blocks = p.row_blocks; x.splits = p.splits;
+        x.shared = shared; x.part0 = part0;
+        if (shared) { x.kv_len = prefix_len; x.kv_lens = nullptr; }
+        launch_pass<HD, MX>(x, p, s);
+    };
+    if (prefix_len) pass(pre, pl.pre, 1, 0);
+    pass(own, pl.own, 0, pl.pre.splits);
+    if (pl.parts > 1)
+        hipLaunchKernelGGL(kv_attention_join_kernel<HD>, dim3((unsigned)((pl.rows * (HD / 4) + 255) / 256)), dim3(256), 0, s, a.o_part, a.ml_part,
+                           pl.rows, pl.parts, a.H, out, a.ldo);
 }
 
 extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq,
                                    void* out, int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale,
                                    int causal, void* workspace, size_t workspace_bytes, void* stream) {
-    AttnArgs a = {};
-    if (const int rc = check_cache("seedmi_kv_attention", cache, &a.c)) return rc;
+    KvView own, pre;
+    if (const int rc = check_cache("seedmi_kv_attention", cache, &own)) return rc;
     const int hd = cache->head_dim, G = cache->kv_heads;
     if (prefix_len < 0 || (prefix_len > 0 && !prefix)) {
         seedmi_set_error("seedmi_kv_attention: prefix_len %d without a prefix", prefix_len);
         return SEEDMI_E_SHAPE;
     }
-    a.p = a.c;
+    pre = own;
     if (prefix_len) {
-        if (const int rc = check_cache("seedmi_kv_attention (prefix)", prefix, &a.p)) return rc;
+        if (const int rc = check_cache("seedmi_kv_attention (prefix)", prefix, &pre)) return rc;
         if (prefix->head_dim != hd || prefix->kv_heads != G || prefix->format != cache->format || prefix_len > prefix->rows) {
             seedmi_set_error("seedmi_kv_attention: the prefix has head_dim %d, %d key heads, format %d, %d rows (%d asked); the cache %d, %d, %d",
                              prefix->head_dim, prefix->kv_heads, prefix->format, prefix->rows, prefix_len, hd, G, cache->format);
@@ -365,9 +764,9 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
         }
     }
     if (!q || !out || B <= 0 || B > cache->slots || T <= 0 || H <= 0 || (H % G) || ldq < (long long)H * hd || ldo < (long long)H * hd ||
-        kv_max < 0 || !(scale == scale)) {
-        seedmi_set_error("seedmi_kv_attention: null pointer or bad shape: B=%d (slots %d) T=%d H=%d (a multiple of %d) ldq=%d ldo=%d kv_max=%d", B,
-                         cache->slots, T, H, G, ldq, ldo, kv_max);
+        kv_max < 0 || !(scale > 0.f) || scale > 3e38f) {
+        seedmi_set_error("seedmi_kv_attention: null pointer or bad shape: B=%d (slots %d) T=%d H=%d (a multiple of %d) ldq=%d ldo=%d kv_max=%d "
+                         "scale=%g (finite, above 0)", B, cache->slots, T, H, G, ldq, ldo, kv_max, scale);
         return SEEDMI_E_SHAPE;
     }
     if (!kv_lens_i32 && (kv_len < 0 || kv_len > cache->rows)) {
@@ -378,22 +777,24 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
         seedmi_set_error("seedmi_kv_attention: pointers 16-byte aligned, leading dimensions multiples of 8");
         return SEEDMI_E_ALIGN;
     }
-    const long long rows = (long long)B * T * H;
-    if (rows > INT_MAX) {
-        seedmi_set_error("seedmi_kv_attention: B * T * H = %lld: at most 2^31 - 1", rows);
+    KvPlan pl;
+    if (make_plan(cache, B, T, H, kv_max, prefix_len, &pl)) {
+        seedmi_set_error("seedmi_kv_attention: B * T * H = %lld: at most 2^31 - 1", (long long)B * T * H);
         return SEEDMI_E_SHAPE;
     }
-    const size_t need = seedmi_kv_attention_workspace_bytes(cache, B, T, H, kv_max, prefix_len);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))) {
-        seedmi_set_error("seedmi_kv_attention: workspace %zu bytes (need %zu, 256-byte aligned)", workspace_bytes, need);
+    if (pl.bytes && (!workspace || workspace_bytes < pl.bytes || ((uintptr_t)workspace & 255))) {
+        seedmi_set_error("seedmi_kv_attention: workspace %zu bytes (need %zu, 256-byte aligned)", workspace_bytes, pl.bytes);
         return SEEDMI_E_ALIGN;
     }
-    a.q = (const bf16_t*)q; a.out = (bf16_t*)out;
-    a.ldq = ldq; a.ldo = ldo; a.B = B; a.T = T; a.H = H;
+    AttnArgs a = {};
+    a.q = (const bf16_t*)q;
+    a.ldq = ldq; a.ldo = ldo; a.T = T; a.H = H; a.GH = H / G;
     a.kv_len = kv_len; a.kv_lens = (const int*)kv_lens_i32;
-    a.prefix_len = prefix_len; a.causal = causal; a.scale = scale;
-#define CALL(HD, MX)                                                                                                            \
-    hipLaunchKernelGGL((kv_attention_rows_kernel<HD, MX>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a)
+    a.causal = causal; a.c2 = scale * 1.44269504088896340736f;
+    a.rows = pl.rows;
+    a.ml_part = (float2*)workspace;
+    a.o_part = (float*)((char*)workspace + (((size_t)pl.parts * pl.rows * 8 + 255) & ~(size_t)255));
+#define CALL(HD, MX) launch_attention<HD, MX>(a, own, pre, pl, prefix_len, (bf16_t*)out, (hipStream_t)stream)
     KV_DISPATCH(hd, cache->format == SEEDMI_KV_MX8, CALL);
 #undef CALL
     return seedmi_check_launch("kv_attention");
