@@ -323,7 +323,7 @@ SEEDMI_DEVINL void lds_fence() { asm volatile("" ::: "memory"); }        // (a w
 // lane's scores are keys 4 g + r of its query li, which is the layout the P^T operand of O^T = V^T P^T needs: P never leaves registers.
 // V is transposed through 8 KiB of LDS that the wave has to itself (no barrier in the loop).
 template <int HD, bool MX, int MT>
-__global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void kv_attention_few_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs a) {
     constexpr int NT = HD / 16, KS = HD / 32;
     constexpr int VBYTES = KT * HD * 2;
     __shared__ __attribute__((aligned(16))) char sm[4 * (VBYTES > 16 * HD * 4 ? VBYTES : 16 * HD * 4)];
@@ -546,30 +546,304 @@ __global__ __launch_bounds__(256, MT == 4 ? 1 : 2) void kv_attention_few_kernel(
     }
 }
 
-// The parts of every row joined: HD / 4 lanes per row.
-template <int HD>
+// ---- many query rows per group (prompt chunks, a prefix that many slots share): bound by the matrix and vector pipes.
+// Workgroup = (group, block of 64 MT rows, key range), wave = 16 MT rows; 64-key tiles of K and V are widened to 16 bits once and shared
+// through a double-buffered LDS image, one barrier per tile; the next tile's bytes are in registers meanwhile, so that neither the load nor
+// the widening sits between two tiles.
+constexpr int KT2 = 64;
+
+template <int HD, bool MX>
+struct Stage {                                           // a thread's part of a 64-key tile of K and of V: HD * 4 / RB rows ... 16 bytes each
+    static constexpr int RB = MX ? HD : 2 * HD;
+    static constexpr int LPR = RB / 16;                  // threads of a row
+    static constexpr int L = KT2 * LPR / 256;            // 16-byte loads per thread and operand
+    uint4 k[L], v[L];
+    uint32_t ks[L], vs[L];
+};
+template <int HD, bool MX>
+SEEDMI_DEVINL void stage_load(Stage<HD, MX>& t, const char* kb, const uint8_t* ksb, const char* vb, const uint8_t* vsb, int key0, int last, int tid) {
+    using S = Stage<HD, MX>;
+#pragma unroll
+    for (int j = 0; j < S::L; ++j) {
+        const long long row = min(key0 + j * (256 / S::LPR) + tid / S::LPR, last);
+        const int c = tid % S::LPR;
+        t.k[j] = *(const uint4*)(kb + row * S::RB + 16 * c);
+        t.v[j] = *(const uint4*)(vb + row * S::RB + 16 * c);
+        if (MX) {
+            t.ks[j] = ksb[row * (HD / 32) + c / 2];
+            t.vs[j] = vsb[row * (HD / 32) + c / 2];
+        }
+    }
+}
+template <int HD, bool MX>
+SEEDMI_DEVINL void stage_store(const Stage<HD, MX>& t, char* kl, char* vl, int tid) {
+    using S = Stage<HD, MX>;
+    auto put = [](char* dst, uint4 w, uint32_t sb, int row, int c) {
+        if (MX) {
+            const float s = mx_scale_f(sb);
+            *(uint4*)(dst + v_chunk<HD>(row, 2 * c)) = make_uint4(mx_unpack2<false>(w.x, s), mx_unpack2<true>(w.x, s), mx_unpack2<false>(w.y, s), mx_unpack2<true>(w.y, s));
+            *(uint4*)(dst + v_chunk<HD>(row, 2 * c + 1)) = make_uint4(mx_unpack2<false>(w.z, s), mx_unpack2<true>(w.z, s), mx_unpack2<false>(w.w, s), mx_unpack2<true>(w.w, s));
+        } else {
+            *(uint4*)(dst + v_chunk<HD>(row, c)) = make_uint4(w.x, w.y, w.z, w.w);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < S::L; ++j) {
+        const int row = j * (256 / S::LPR) + tid / S::LPR, c = tid % S::LPR;
+        put(kl, t.k[j], MX ? t.ks[j] : 0u, row, c);
+        put(vl, t.v[j], MX ? t.vs[j] : 0u, row, c);
+    }
+}
+
+template <int HD, bool MX, int MT>
+__global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArgs a) {
+    constexpr int NT = HD / 16, KS = HD / 32;
+    constexpr int TB = KT2 * HD * 2;                     // bytes of a widened tile
+    __shared__ __attribute__((aligned(16))) char sm[4 * TB];             // K0 K1 V0 V1
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned items = (unsigned)a.groups * a.splits;
+    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    const unsigned item = blk * 8 + in % 8;
+    const int rb = a.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
+    if (item >= items) return;
+    const int split = item / a.groups, group = item % a.groups;
+    const int G = a.c.G, slot = group / G, kvh = group % G;
+    const int base = a.shared ? 0 : slot * a.T;
+    const int r0 = rb * 64 * MT, r_end = min(a.group_rows, r0 + 64 * MT);
+
+    int len = a.kv_len;
+    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
+    len = max(0, min(len, a.c.rows));
+    const bool causal = a.causal && !a.shared;
+    const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
+    const int tiles = (n_max + KT2 - 1) / KT2;
+    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int t_begin = split * per, t_end = min(tiles, t_begin + per);
+    // what the rows of this wave see at least and at most (its rows may lie beyond the group's end)
+    const int w0 = r0 + 16 * MT * wave, w1 = min(r_end - 1, w0 + 16 * MT - 1);
+    const int wave_max = w0 >= r_end ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
+    const int wave_min = w0 >= r_end ? 0 : causal ? len - a.T + w0 / a.GH + 1 : len;
+
+    bf16x8 qf[MT][KS];
+    int seen[MT];
+    float m[MT], l[MT];
+    f32x4 o[MT][NT];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const int r = w0 + 16 * u + li;
+        const bool on = r < r_end;
+        seen[u] = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
+        const bf16_t* qp = a.q + (size_t)(base + (on ? r / a.GH : 0)) * a.ldq + (kvh * a.GH + (on ? r % a.GH : 0)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (on) v = *(const uint4*)(qp + 32 * ks + 8 * g4);
+            qf[u][ks] = __builtin_bit_cast(bf16x8, v);
+        }
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    using S = Stage<HD, MX>;
+    const char* kb = a.c.k + row0 * S::RB;
+    const char* vb = a.c.v + row0 * S::RB;
+    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    const int last = n_max - 1;
+
+    S st;
+    if (t_begin < t_end) {
+        stage_load(st, kb, ksb, vb, vsb, t_begin * KT2, last, tid);
+        stage_store(st, sm, sm + 2 * TB, tid);
+        stage_load(st, kb, ksb, vb, vsb, min(t_begin + 1, t_end - 1) * KT2, last, tid);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int tile = t_begin; tile < t_end; ++tile) {
+        const int key0 = tile * KT2, cur = (tile - t_begin) & 1;
+        char* kl = sm + cur * TB;
+        char* vl = sm + (2 + cur) * TB;
+        bool mixed = false;
+        if (key0 + KT2 > n_max || (causal && key0 + KT2 > len - a.T + r0 / a.GH + 1)) {          // (uniform) some row does not see it all
+            bool bad = false;
+#pragma unroll 1
+            for (int i = 4 * tid; i < TB; i += 1024) {
+                const uint32_t x = *(const uint32_t*)(vl + i);
+                bad |= bad16(x & 0xffffu) | bad16(x >> 16);
+            }
+            mixed = __syncthreads_or(bad) != 0;
+        }
+        f32x4 s[MT][4];
+        const bool live = key0 < wave_max;               // (wave-uniform)
+        if (live) {
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                bf16x8 kf[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + v_chunk<HD>(16 * kt + li, 4 * ks + g4));
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) s[u][kt] = seedmi_mfma_16x16x32(kf[ks], qf[u][ks], s[u][kt]);
+                }
+            }
+        }
+        // the next tile into the other buffer (read last before the barrier that ended the previous tile), the one after it requested
+        if (tile + 1 < t_end) {
+            stage_store(st, sm + (cur ^ 1) * TB, sm + (2 + (cur ^ 1)) * TB, tid);
+            stage_load(st, kb, ksb, vb, vsb, min(tile + 2, t_end - 1) * KT2, last, tid);
+        }
+        bf16x8 pf[MT][2];
+        if (live) {
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                if (key0 + KT2 > wave_min) {
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (key0 + 16 * kt + 4 * g4 + r >= seen[u]) s[u][kt][r] = -INFINITY;
+                }
+                float tm = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) tm = fmaxf(tm, fmaxf(fmaxf(s[u][kt][0], s[u][kt][1]), fmaxf(s[u][kt][2], s[u][kt][3])));
+                tm = rows_max(tm) * a.c2;
+                const float mn = fmaxf(m[u], tm);
+                if (__any(mn > m[u])) {
+                    const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
+                    l[u] *= f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
+                    m[u] = mn;
+                }
+                const float ref = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        p[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                        l[u] += p[j];
+                    }
+                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])));
+                }
+            }
+        }
+        if (mixed) {                                     // see kv_attention_few_kernel
+            if (live) {
+#pragma unroll 1
+                for (int j = 0; j < KT2; ++j) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint2 w = *(const uint2*)(vl + v_chunk<HD>(j, 2 * n + (g4 >> 1)) + 8 * (g4 & 1));
+                        const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int u = 0; u < MT; ++u)
+                                if (bad16(h[r]) && key0 + j < seen[u]) o[u][n][r] += bf2f((bf16_t)h[r]);
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 4 * tid; i < TB; i += 1024) {
+                const uint32_t x = *(uint32_t*)(vl + i), lo = x & 0xffffu, hi = x >> 16;
+                *(uint32_t*)(vl + i) = (bad16(lo) ? 0u : lo) | ((bad16(hi) ? 0u : hi) << 16);
+            }
+            __syncthreads();
+        }
+        if (live) {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const bf16x8 vf = v_frag<HD>(vl + kk * (32 * 2 * HD), n, lane);
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) o[u][n] = seedmi_mfma_16x16x32(vf, pf[u][kk], o[u][n]);
+                }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const float L = rows_sum(l[u]);
+        const int r = w0 + 16 * u + li;
+        if (r >= r_end) continue;
+        const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
+        if (a.out) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                *(uint2*)(op + 16 * n) = make_uint2(pack2bf(o[u][n][0] * inv, o[u][n][1] * inv), pack2bf(o[u][n][2] * inv, o[u][n][3] * inv));
+        } else {
+            const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
+            if (L != 0.f) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) *(f32x4*)(a.o_part + at * HD + 16 * n + 4 * g4) = o[u][n];
+            }
+            if (g4 == 0) a.ml_part[at] = make_float2(fmaxf(m[u], LOWEST), L);
+        }
+    }
+}
+
+// The parts of every row joined.  Thread = 4 channels of a row and every JW-th of its parts (few rows have many parts: a thread that walked
+// them all would wait for one memory round trip after the other); the JW partial sums meet in the LDS.
+template <int HD, int JW>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml, long long rows,
                                                                 int parts, int H, bf16_t* __restrict__ out, int ldo) {
-    constexpr int LPR = HD / 4;
-    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
-    if (row >= rows) return;
-    const int d = 4 * (threadIdx.x % LPR);
-    float M = LOWEST;
-    for (int p = 0; p < parts; ++p) M = fmaxf(M, ml[p * rows + row].x);
-    float L = 0.f;
+    constexpr int LPR = HD / 4, RPB = 256 / (LPR * JW);  // threads of a row's channels, rows of a workgroup
+    const int c = threadIdx.x % LPR, w = (threadIdx.x / LPR) % JW, lr = threadIdx.x / (LPR * JW);
+    const long long row = (long long)blockIdx.x * RPB + lr;
+    const bool on = row < rows;
+    float M = LOWEST, L = 0.f;
     f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-        const float2 x = ml[p * rows + row];
-        if (x.y == 0.f) continue;                        // (a NaN sum is not skipped)
-        const float f = exp2_hw(x.x - M);
-        L += x.y * f;
-        const f32x4 v = *(const f32x4*)(o_part + (p * rows + row) * HD + d);
+    if (on) {
+#pragma unroll 4
+        for (int p = w; p < parts; p += JW) {
+            const float2 x = ml[p * rows + row];
+            if (x.y == 0.f) continue;                    // nothing there (a NaN sum is not skipped)
+            const f32x4 v = *(const f32x4*)(o_part + (p * rows + row) * HD + 4 * c);
+            const float mn = fmaxf(M, x.x);
+            const float f0 = exp2_hw(M - mn), f1 = exp2_hw(x.x - mn);
+            M = mn;
+            L = L * f0 + x.y * f1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += v[i] * f;
+            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
+        }
     }
+    if (JW > 1) {
+        __shared__ f32x4 so[JW > 1 ? 256 : 1];
+        __shared__ float2 sl[JW > 1 ? 256 : 1];
+        so[threadIdx.x] = o;
+        sl[threadIdx.x] = make_float2(M, L);
+        __syncthreads();
+        if (w || !on) return;
+#pragma unroll
+        for (int k = 1; k < JW; ++k) {
+            const float2 x = sl[threadIdx.x + k * LPR];
+            if (x.y == 0.f) continue;
+            const f32x4 v = so[threadIdx.x + k * LPR];
+            const float mn = fmaxf(M, x.x);
+            const float f0 = exp2_hw(M - mn), f1 = exp2_hw(x.x - mn);
+            M = mn;
+            L = L * f0 + x.y * f1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
+        }
+    }
+    if (!on) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int token = (int)(row / H), head = (int)(row % H);
-    *(uint2*)(out + (size_t)token * ldo + head * HD + d) = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
+    *(uint2*)(out + (size_t)token * ldo + head * HD + 4 * c) = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -677,17 +951,20 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
 }
 
 // How a call is cut: a pass over the slots' own rows and, with a prefix, one over the prefix; row blocks and key ranges of each.
-struct KvPass { int groups, group_rows, mt, row_blocks, splits; };
+struct KvPass { int groups, group_rows, block_rows, row_blocks, splits; };
 struct KvPlan { KvPass own, pre; int parts; long long rows; size_t bytes; };
 
 static KvPass plan_pass(int groups, long long rows, long long keys) {
     KvPass p = {};
     p.groups = groups;
     p.group_rows = (int)rows;
-    p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    p.row_blocks = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
-    const long long tiles = (keys + KT - 1) / KT, base = (long long)groups * p.row_blocks;
-    long long s = (1024 + base - 1) / base;
+    // up to 32 rows: the few-rows kernel with one or two blocks of 16; beyond: the many-rows kernel, 64 or 128 to a workgroup
+    p.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
+    const int kt = p.block_rows <= 32 ? KT : KT2;
+    const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
+    const long long target = p.block_rows == 16 ? 768 : 512;              // workgroups that the 256 CUs hold at once
+    long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
@@ -719,11 +996,19 @@ template <int HD, bool MX>
 static void launch_pass(const AttnArgs& a, const KvPass& p, hipStream_t s) {
     const unsigned items = (unsigned)p.groups * p.splits;
     const dim3 grid((items + 7) / 8 * 8 * p.row_blocks);
-    switch (p.mt) {
-        case 1: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
-        case 2: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 4>), grid, dim3(256), 0, s, a); break;
+    switch (p.block_rows) {
+        case 16: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
+        case 32: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
     }
+}
+
+template <int HD, int JW>
+static void launch_join(const AttnArgs& a, const KvPlan& pl, bf16_t* out, hipStream_t s) {
+    constexpr int RPB = 256 / (HD / 4 * JW);
+    hipLaunchKernelGGL((kv_attention_join_kernel<HD, JW>), dim3((unsigned)((pl.rows + RPB - 1) / RPB)), dim3(256), 0, s, a.o_part, a.ml_part,
+                       pl.rows, pl.parts, a.H, out, a.ldo);
 }
 
 template <int HD, bool MX>
@@ -739,9 +1024,8 @@ static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, c
     };
     if (prefix_len) pass(pre, pl.pre, 1, 0);
     pass(own, pl.own, 0, pl.pre.splits);
-    if (pl.parts > 1)
-        hipLaunchKernelGGL(kv_attention_join_kernel<HD>, dim3((unsigned)((pl.rows * (HD / 4) + 255) / 256)), dim3(256), 0, s, a.o_part, a.ml_part,
-                           pl.rows, pl.parts, a.H, out, a.ldo);
+    if (pl.parts > 4) launch_join<HD, 8>(a, pl, out, s);
+    else if (pl.parts > 1) launch_join<HD, 1>(a, pl, out, s);
 }
 
 extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq,
