@@ -229,6 +229,10 @@ SEEDMI_DEVINL uint32_t exp_mask16() {
 #endif
 }
 SEEDMI_DEVINL bool bad16(uint32_t h) { return (h & exp_mask16()) == exp_mask16(); }
+SEEDMI_DEVINL bool bad_word(uint32_t w) { return bad16(w) | bad16(w >> 16); }
+SEEDMI_DEVINL bool bad_words(const uint4& w) { return bad_word(w.x) | bad_word(w.y) | bad_word(w.z) | bad_word(w.w); }
+// zeros in place of what is not finite
+SEEDMI_DEVINL uint32_t clean_word(uint32_t w) { return (bad16(w) ? 0u : w & 0xffffu) | (bad16(w >> 16) ? 0u : w & 0xffff0000u); }
 
 // A tile of 32 keys and values as a wave holds it between the load and its use.
 //   K (the MFMA's A operand, rows = keys): lane (li, g) holds its part of rows 16 kt + li.  16-bit rows: k-step ks = values 32 ks + 8 g ..;
@@ -289,14 +293,14 @@ SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int rows, int lane)
             for (int d = 0; d < 4; ++d) {
                 o[2 * d] = mx_unpack2<false>(src[d], s);
                 o[2 * d + 1] = mx_unpack2<true>(src[d], s);
-                if (TAIL) bad |= bad16(o[2 * d] & 0xffffu) | bad16(o[2 * d] >> 16) | bad16(o[2 * d + 1] & 0xffffu) | bad16(o[2 * d + 1] >> 16);
+                if (TAIL) bad |= bad_word(o[2 * d]) | bad_word(o[2 * d + 1]);
             }
             *(uint4*)(lds + v_chunk<HD>(row, 2 * l)) = make_uint4(o[0], o[1], o[2], o[3]);
             *(uint4*)(lds + v_chunk<HD>(row, 2 * l + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         } else {
 #pragma unroll
             for (int d = 0; d < 4; ++d)
-                if (TAIL) bad |= bad16(src[d] & 0xffffu) | bad16(src[d] >> 16);
+                if (TAIL) bad |= bad_word(src[d]);
             *(uint4*)(lds + v_chunk<HD>(row, l)) = w;
         }
     }
@@ -477,10 +481,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs
             for (int i = 16 * lane; i < VBYTES; i += 1024) {
                 uint32_t* w = (uint32_t*)(lds + i);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t x = w[d], lo = x & 0xffffu, hi = x >> 16;
-                    w[d] = (bad16(lo) ? 0u : lo) | ((bad16(hi) ? 0u : hi) << 16);
-                }
+                for (int d = 0; d < 4; ++d) w[d] = clean_word(w[d]);
             }
             lds_fence();
         }
@@ -671,8 +672,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             bool bad = false;
 #pragma unroll 1
             for (int i = 4 * tid; i < TB; i += 1024) {
-                const uint32_t x = *(const uint32_t*)(vl + i);
-                bad |= bad16(x & 0xffffu) | bad16(x >> 16);
+                bad |= bad_word(*(const uint32_t*)(vl + i));
             }
             mixed = __syncthreads_or(bad) != 0;
         }
@@ -754,8 +754,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             __syncthreads();
 #pragma unroll 1
             for (int i = 4 * tid; i < TB; i += 1024) {
-                const uint32_t x = *(uint32_t*)(vl + i), lo = x & 0xffffu, hi = x >> 16;
-                *(uint32_t*)(vl + i) = (bad16(lo) ? 0u : lo) | ((bad16(hi) ? 0u : hi) << 16);
+                *(uint32_t*)(vl + i) = clean_word(*(uint32_t*)(vl + i));
             }
             __syncthreads();
         }
@@ -789,6 +788,270 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             if (L != 0.f) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) *(f32x4*)(a.o_part + at * HD + 16 * n + 4 * g4) = o[u][n];
+            }
+            if (g4 == 0) a.ml_part[at] = make_float2(fmaxf(m[u], LOWEST), L);
+        }
+    }
+}
+
+// ---- hundreds of query rows per group: bound by the matrix pipe, with the vector pipe (softmax) and the LDS close behind.
+// Workgroup = (group, block of 256 rows, key range), two halves of four waves; wave = 32 rows.  A tile costs a wave a MATRIX phase (the product
+// with the previous tile's values, then the scores of this one: 68 MFMAs) and a VECTOR phase (softmax, staging) of about the same length.
+// The halves run one phase apart, so that on every SIMD one wave is in its matrix phase while the other is in its vector phase; a barrier
+// ends each phase.  Phase 2 t: half 0 multiplies (values of t - 1, keys of t); phase 2 t + 1: half 1 does.  Keys of tile t are read in
+// phases 2 t and 2 t + 1, values in 2 t + 2 and 2 t + 3; each half stages its 32 rows of a tile in its vector phases: half h, after the
+// scores of tile t, keys of t + 1 + h and values of t + h - two LDS buffers each, always written after their last reader's barrier.
+// The row sums come from the matrix pipe as well (a product of P with ones: 4 of the 68 MFMAs instead of 32 additions).
+template <int HD, bool MX>
+struct HalfStage {                                       // a thread's part of 32 rows of K and V
+    static constexpr int RB = MX ? HD : 2 * HD;
+    static constexpr int LPR = RB / 16;
+    static constexpr int L = (32 * LPR + 255) / 256;     // 16-byte loads per thread (8-bit rows of 64: by half of the threads)
+    uint4 k[L], v[L];
+    uint32_t ks[L], vs[L];
+};
+
+template <int HD, bool MX>
+__global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs a) {
+    constexpr int MT = 2, NT = HD / 16, KS = HD / 32;
+    constexpr int TB = KT2 * HD * 2;
+    __shared__ __attribute__((aligned(16))) char sm[6 * TB];             // K0 K1 V0 V1, raw V0 V1
+    __shared__ int s_bad;                                // a tile that some row does not see whole held a value that is not finite
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, ht = tid & 255;
+    const unsigned items = (unsigned)a.groups * a.splits;
+    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    const unsigned item = blk * 8 + in % 8;
+    const int rb = a.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
+    if (item >= items) return;
+    const int split = item / a.groups, group = item % a.groups;
+    const int G = a.c.G, slot = group / G, kvh = group % G;
+    const int base = a.shared ? 0 : slot * a.T;
+    const int r0 = rb * 256, r_end = min(a.group_rows, r0 + 256);
+
+    int len = a.kv_len;
+    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
+    len = max(0, min(len, a.c.rows));
+    const bool causal = a.causal && !a.shared;
+    const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
+    const int n_min = causal ? len - a.T + r0 / a.GH + 1 : len;
+    const int tiles = (n_max + KT2 - 1) / KT2;
+    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int t0 = split * per, n = max(0, min(tiles, t0 + per) - t0);   // first tile, number of tiles
+    const int w0 = r0 + 32 * wave, w1 = min(r_end - 1, w0 + 31);
+    const int wave_max = w0 >= r_end ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
+    const int wave_min = w0 >= r_end ? 0 : causal ? len - a.T + w0 / a.GH + 1 : len;
+
+    bf16x8 qf[MT][KS];
+    int seen[MT];
+    float m[MT];
+    f32x4 o[MT][NT], l[MT];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const int r = w0 + 16 * u + li;
+        const bool on = r < r_end;
+        seen[u] = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
+        const bf16_t* qp = a.q + (size_t)(base + (on ? r / a.GH : 0)) * a.ldq + (kvh * a.GH + (on ? r % a.GH : 0)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (on) v = *(const uint4*)(qp + 32 * ks + 8 * g4);
+            qf[u][ks] = __builtin_bit_cast(bf16x8, v);
+        }
+        m[u] = -INFINITY;
+        l[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[u][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    using S = HalfStage<HD, MX>;
+    const char* kb = a.c.k + row0 * S::RB;
+    const char* vb = a.c.v + row0 * S::RB;
+    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    const int last = n_max - 1;
+    const int srow = 32 * half + ht / S::LPR, schunk = ht % S::LPR;      // the thread's first row of a tile and its 16-byte piece of it
+    const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
+
+    S st;
+    auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const char* b, const uint8_t* sb, int t) {
+        if (!stages) return;
+#pragma unroll
+        for (int j = 0; j < S::L; ++j) {
+            const long long row = min((t0 + min(t, n - 1)) * KT2 + srow + j * (256 / S::LPR), last);
+            w[j] = *(const uint4*)(b + row * S::RB + 16 * schunk);
+            if (MX) sc[j] = sb[row * (HD / 32) + schunk / 2];
+        }
+    };
+    // raw: where a value tile that some row does not see whole leaves its rows as they are; the image then holds zeros in place of what is not
+    // finite (0 * inf must not reach a row that does not see the key; the rows that do take it from the raw rows)
+    auto store_rows = [&](const uint4 (&w)[S::L], const uint32_t (&sc)[S::L], char* dst, char* raw) {
+        if (!stages) return;
+        bool bad = false;
+        auto put = [&](int at, uint4 x) {
+            if (raw) {
+                *(uint4*)(raw + at) = x;
+                bad |= bad_words(x);
+                x = make_uint4(clean_word(x.x), clean_word(x.y), clean_word(x.z), clean_word(x.w));
+            }
+            *(uint4*)(dst + at) = x;
+        };
+#pragma unroll
+        for (int j = 0; j < S::L; ++j) {
+            const int row = srow + j * (256 / S::LPR);
+            if (MX) {
+                const float s = mx_scale_f(sc[j]);
+                put(v_chunk<HD>(row, 2 * schunk), make_uint4(mx_unpack2<false>(w[j].x, s), mx_unpack2<true>(w[j].x, s), mx_unpack2<false>(w[j].y, s), mx_unpack2<true>(w[j].y, s)));
+                put(v_chunk<HD>(row, 2 * schunk + 1), make_uint4(mx_unpack2<false>(w[j].z, s), mx_unpack2<true>(w[j].z, s), mx_unpack2<false>(w[j].w, s), mx_unpack2<true>(w[j].w, s)));
+            } else {
+                put(v_chunk<HD>(row, schunk), make_uint4(w[j].x, w[j].y, w[j].z, w[j].w));
+            }
+        }
+        if (raw && bad) s_bad = 1;
+    };
+    auto kbuf = [&](int t) { return sm + (t & 1) * TB; };
+    auto vbuf = [&](int t) { return sm + (2 + (t & 1)) * TB; };
+    auto mixed_tile = [&](int t) { return (t0 + t + 1) * KT2 > n_min; }; // some row of the block does not see all of it
+    auto vraw = [&](int t) { return mixed_tile(t) ? sm + (4 + (t & 1)) * TB : nullptr; };
+
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    if (n > 0) {
+        load_rows(st.k, st.ks, kb, ksb, 0);
+        store_rows(st.k, st.ks, kbuf(0), nullptr);
+        if (half) {                                      // half 1 is one vector phase ahead in its staging
+            load_rows(st.k, st.ks, kb, ksb, 1);
+            load_rows(st.v, st.vs, vb, vsb, 0);
+            if (n > 1) store_rows(st.k, st.ks, kbuf(1), nullptr);
+            store_rows(st.v, st.vs, vbuf(0), vraw(0));
+        }
+        load_rows(st.k, st.ks, kb, ksb, 1 + half);
+        load_rows(st.v, st.vs, vb, vsb, half);
+    }
+    __syncthreads();
+
+    bf16x8 pf[MT][2];
+    auto values = [&](int t) {                           // o += P V, l += P 1 for the tile whose probabilities are in pf
+        const char* vl = vbuf(t);
+        const bf16x8 ones = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(1.f, 1.f), pack2bf(1.f, 1.f), pack2bf(1.f, 1.f), pack2bf(1.f, 1.f)));
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const bf16x8 vf = v_frag<HD>(vl + kk * (32 * 2 * HD), i, lane);
+#pragma unroll
+                for (int u = 0; u < MT; ++u) o[u][i] = seedmi_mfma_16x16x32(vf, pf[u][kk], o[u][i]);
+            }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int u = 0; u < MT; ++u) l[u] = seedmi_mfma_16x16x32(ones, pf[u][kk], l[u]);
+        if (__builtin_expect(mixed_tile(t) && __builtin_amdgcn_readfirstlane(s_bad), 0)) {
+            const char* rl = sm + (4 + (t & 1)) * TB;
+#pragma unroll 1
+            for (int j = 0; j < KT2; ++j) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const uint2 w = *(const uint2*)(rl + v_chunk<HD>(j, 2 * i + (g4 >> 1)) + 8 * (g4 & 1));
+                    const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int u = 0; u < MT; ++u)
+                            if (bad16(h[r]) && (t0 + t) * KT2 + j < seen[u]) o[u][i][r] += bf2f((bf16_t)h[r]);
+                }
+            }
+        }
+    };
+
+    if (half) __syncthreads();                           // phase 0 belongs to half 0
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+        const int key0 = (t0 + t) * KT2;
+        // ---- matrix phase
+        __builtin_amdgcn_s_setprio(1);
+        f32x4 s[MT][4];
+        const bool live = key0 < wave_max;               // (wave-uniform; tiles are in order: once dead, dead to the end)
+        if (t > 0 && key0 - KT2 < wave_max) values(t - 1);
+        if (live) {
+            const char* kl = kbuf(t);
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                bf16x8 kf[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + v_chunk<HD>(16 * kt + li, 4 * ks + g4));
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) s[u][kt] = seedmi_mfma_16x16x32(kf[ks], qf[u][ks], s[u][kt]);
+                }
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        __syncthreads();
+        // ---- vector phase
+        if (t + 1 + half < n) store_rows(st.k, st.ks, kbuf(t + 1 + half), nullptr);
+        if (t + half < n) store_rows(st.v, st.vs, vbuf(t + half), vraw(t + half));
+        load_rows(st.k, st.ks, kb, ksb, t + 2 + half);
+        load_rows(st.v, st.vs, vb, vsb, t + 1 + half);
+        if (live) {
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                if (key0 + KT2 > wave_min) {
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (key0 + 16 * kt + 4 * g4 + r >= seen[u]) s[u][kt][r] = -INFINITY;
+                }
+                float tm = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) tm = fmaxf(tm, fmaxf(fmaxf(s[u][kt][0], s[u][kt][1]), fmaxf(s[u][kt][2], s[u][kt][3])));
+                tm = rows_max(tm) * a.c2;
+                const float mn = fmaxf(m[u], tm);
+                if (__any(mn > m[u])) {
+                    const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) l[u][r] *= f;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[u][i][r] *= f;
+                    m[u] = mn;
+                }
+                const float ref = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) p[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])));
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (n > 0 && (t0 + n - 1) * KT2 < wave_max) values(n - 1);
+    if (!half) __syncthreads();                          // (half 1's last vector phase)
+
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const float L = l[u][0];
+        const int r = w0 + 16 * u + li;
+        if (r >= r_end) continue;
+        const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
+        if (a.out) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                *(uint2*)(op + 16 * i) = make_uint2(pack2bf(o[u][i][0] * inv, o[u][i][1] * inv), pack2bf(o[u][i][2] * inv, o[u][i][3] * inv));
+        } else {
+            const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
+            if (L != 0.f) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) *(f32x4*)(a.o_part + at * HD + 16 * i + 4 * g4) = o[u][i];
             }
             if (g4 == 0) a.ml_part[at] = make_float2(fmaxf(m[u], LOWEST), L);
         }
@@ -959,11 +1222,11 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     p.groups = groups;
     p.group_rows = (int)rows;
     // up to 32 rows: the few-rows kernel with one or two blocks of 16; beyond: the many-rows kernel, 64 or 128 to a workgroup
-    p.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    p.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     const int kt = p.block_rows <= 32 ? KT : KT2;
     const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
-    const long long target = p.block_rows == 16 ? 768 : 512;              // workgroups that the 256 CUs hold at once
+    const long long target = p.block_rows == 16 ? 768 : p.block_rows == 256 ? 256 : 512;              // workgroups that the 256 CUs hold at once
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);
@@ -1000,7 +1263,8 @@ static void launch_pass(const AttnArgs& a, const KvPass& p, hipStream_t s) {
         case 16: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
         case 32: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
         case 64: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
+        case 128: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((kv_attention_phased_kernel<HD, MX>), grid, dim3(512), 0, s, a); break;
     }
 }
 

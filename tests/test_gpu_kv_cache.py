@@ -224,6 +224,10 @@ CASES = [  # H, G, D, T, lengths, prefix, causal
     (5, 1, 128, 20, [20, 64], 64, True),
     (2, 2, 128, 140, [140, 150], 77, True),
     (4, 2, 64, 131, [131, 20], 129, True),
+    (4, 4, 128, 64, [64, 200, 30], 0, True),
+    (12, 4, 64, 27, [27, 64, 3], 65, True),
+    (8, 2, 128, 100, [100, 164, 64], 0, True),
+    (3, 1, 128, 171, [171, 172], 0, True),
 ]
 
 
@@ -279,7 +283,7 @@ def test_attention_over_long_caches(fmt, H, G, T, lens, P):
 
 
 @pytest.mark.parametrize("fmt", ["mx8", "16"])
-@pytest.mark.parametrize("T,P", [(4, 0), (20, 40), (150, 0)])
+@pytest.mark.parametrize("T,P", [(4, 0), (12, 0), (20, 40), (50, 0), (150, 0)])
 def test_rows_a_query_does_not_see_have_no_influence(fmt, T, P):
     """NaN in the last rows (16 bits: infinities too): the queries before them are as if the rows were not there, the ones that see them NaN."""
     H, G, D, n = 4, 2, 128, 170
