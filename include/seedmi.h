@@ -318,9 +318,11 @@ int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int
  * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the
  * probabilities (unnormalised, 0 .. 1) are rounded to the 16-bit element for the product with the values.
  * kv_max: the longest n_b expected (0: cache->rows); it decides how the keys are split over workgroups and never what is computed.
- * workspace: seedmi_kv_attention_workspace_bytes() bytes (may be 0), 256-byte aligned; needs no initialisation and carries nothing from one
- * call to the next; calls that may overlap need one each. */
+ * workspace: seedmi_kv_attention_workspace_bytes() bytes (may be 0), 256-byte aligned, initialised once after allocation by
+ * seedmi_kv_attention_workspace_init (stream-ordered: its first 4 KiB are arrival counters, which every call leaves at zero again; the rest
+ * may hold anything).  One workspace serves any calls whose bytes it covers, one after the other; calls that may overlap need one each. */
 size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* cache, int B, int T, int H, int kv_max, int prefix_len);
+int seedmi_kv_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
 int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq, void* out,
                         int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale, int causal,
                         void* workspace, size_t workspace_bytes, void* stream);

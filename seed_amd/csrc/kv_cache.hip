@@ -186,20 +186,38 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, bf16_t* __
 //
 // With s_j = c q.k_j (c = scale * log2 e) a range of keys gives m = max s_j, l = sum 2^(s_j - m), o = sum 2^(s_j - m) v_j; ranges join by
 // M = max m, (l, o) = sum 2^(m - M) (l, o), and out = o / l.
-struct AttnArgs {
+struct AttnPass {                                       // one pass: the slots' own rows, or the shared prefix
     KvView c;                                            // the slots' cache, or the prefix as a cache of one slot
-    const bf16_t* q;
-    bf16_t* out;                                         // direct output (one part only), else NULL
-    float* o_part;                                       // [parts][B*T*H][HD] sums of a part
-    float2* ml_part;                                     // [parts][B*T*H] (m, l); l == 0: the part holds nothing for the row
     const int* kv_lens;
-    int ldq, ldo, T, H, GH, kv_len, causal;
-    int groups, group_rows, row_blocks;                  // groups = slots * G of this pass, rows of a group, blocks of 16 MT rows
-    int shared;                                          // 1: the groups are those of the prefix (kv_len rows, all visible)
-    int splits, part0;                                   // key ranges of this pass and the first one's part index
+    int kv_len, shared;                                  // shared: the groups are those of the prefix (kv_len rows, all visible)
+    int groups, group_rows, row_blocks;                  // groups = slots * G (prefix: G), rows of a group, row blocks of a group
+    int splits, part0;                                   // key ranges and the first one's part index
+    unsigned blocks;                                     // workgroups of the pass
+};
+struct AttnArgs {
+    const bf16_t* q;
+    bf16_t* out;
+    float* o_part;                                       // [parts][B*T*H][HD] sums of a part; parts == 1: unused, results go to out
+    float2* ml_part;                                     // [parts][B*T*H] (m, l); l == 0: the part holds nothing for the row
+    unsigned* arrivals;                                  // one counter per unit that is joined (join_in_place), else NULL
+    int ldq, ldo, T, H, GH, causal, parts;
+    unsigned unit_blocks;                                // workgroups that arrive at a unit's counter
+    int unit_rows;                                       // rows of a unit where it is a whole key head (two passes), else 0
     long long rows;                                      // B * T * H
     float c2;
+    AttnPass pass[2];
 };
+// The pass a workgroup belongs to, field by field (scalar selects; an indexed kernel argument would be copied to memory).
+SEEDMI_DEVINL AttnPass pass_of(const AttnArgs& a, unsigned& block) {
+    const bool second = blockIdx.x >= a.pass[0].blocks;
+    block = blockIdx.x - (second ? a.pass[0].blocks : 0u);
+    AttnPass p;
+#define SEL(f) p.f = second ? a.pass[1].f : a.pass[0].f
+    SEL(c.k); SEL(c.v); SEL(c.ks); SEL(c.vs); SEL(c.slot_rows); SEL(c.head_rows); SEL(c.rows); SEL(c.G);
+    SEL(kv_lens); SEL(kv_len); SEL(shared); SEL(groups); SEL(group_rows); SEL(row_blocks); SEL(splits); SEL(part0); SEL(blocks);
+#undef SEL
+    return p;
+}
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr int KT = 32;                                   // keys of a tile
@@ -318,8 +336,106 @@ SEEDMI_DEVINL bf16x8 v_frag(const char* lds, int n, int lane) {
     return __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y));
 }
 
+// The values are used here: the wait for their loads ends before a loop, whose own waits then count only the loads of its tiles (a wait that
+// also covers these would be a wait for everything in flight, in every iteration).
+template <int N, int M>
+SEEDMI_DEVINL void arrived(bf16x8 (&x)[N][M]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < M; ++j) asm volatile("" : "+v"(x[i][j]));
+}
 constexpr float LOWEST = -3.4028234e38f;
 SEEDMI_DEVINL void lds_fence() { asm volatile("" ::: "memory"); }        // (a wave's own LDS accesses are executed in order)
+
+// ---- joining the parts of a row
+// (m, l, o) of a running join with one more part.  M starts at LOWEST, L and o at zero.
+SEEDMI_DEVINL void join_part(float& M, float& L, f32x4& o, float m, float l, const f32x4& v) {
+    if (l == 0.f) return;                                // nothing there (a NaN sum is not skipped)
+    const float mn = fmaxf(M, m), f0 = exp2_hw(M - mn), f1 = exp2_hw(m - mn);
+    M = mn;
+    L = L * f0 + l * f1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
+}
+SEEDMI_DEVINL void store_row_quad(bf16_t* dst, float L, const f32x4& o) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *(uint2*)dst = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
+}
+// Parts that another workgroup of the same launch will read, maybe on another XCD with an L2 of its own: device-scope accesses, which go past
+// the L2s on both sides.
+SEEDMI_DEVINL void store_pair(float* p, float x, float y, bool device) {
+    if (device) {
+        const unsigned long long w = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+        __hip_atomic_store((unsigned long long*)p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+        *(float2*)p = make_float2(x, y);
+    }
+}
+SEEDMI_DEVINL void store_quad(float* p, const f32x4& v, bool device) {
+    if (device) {
+        store_pair(p, v[0], v[1], true);
+        store_pair(p + 2, v[2], v[3], true);
+    } else {
+        *(f32x4*)p = v;
+    }
+}
+SEEDMI_DEVINL float2 load_pair(const float* p) {
+    const unsigned long long w = __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
+}
+// The last workgroup of a unit to get here joins the unit's rows, in the order of their parts whoever is last: no second launch.  Rows
+// first .. + n of the group that starts at token `base`, key head kvh.  Every part's stores are past the L2s (waited for) before the
+// workgroup's arrival is counted; the counter wraps to zero with the last arrival.  Workgroups wait for nobody.
+template <int HD>
+SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh, int first, int n, float* lds) {
+    constexpr int LPR = HD / 4, SLOTS = 256 / LPR, BATCH = 4;
+    __shared__ unsigned s_last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's stores have reached memory ...
+    __syncthreads();                                     // ... and so have the other waves'
+    if (threadIdx.x == 0) s_last = atomicInc(a.arrivals + unit, a.unit_blocks - 1) == a.unit_blocks - 1;
+    __syncthreads();
+    if (!s_last) return;
+    asm volatile("" ::: "memory");
+    const int c = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    int jw = SLOTS;                                      // threads that share a row's parts: all of them for one row, one each from SLOTS rows on
+    while (jw > 1 && jw * n > SLOTS) jw >>= 1;
+    const int w = slot % jw, rows_at_once = SLOTS / jw;
+    for (int i0 = 0; i0 < n; i0 += rows_at_once) {
+        const int r = first + i0 + slot / jw;
+        const bool on = r < first + n;
+        const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
+        const long long row = (long long)token * a.H + head;
+        float M = LOWEST, L = 0.f;
+        f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (on) {
+            for (int q = w; q < a.parts; q += BATCH * jw) {
+                float2 ml[BATCH], x[BATCH], y[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const long long at = (long long)min(q + k * jw, a.parts - 1) * a.rows + row;
+                    ml[k] = load_pair((const float*)(a.ml_part + at));
+                    x[k] = load_pair(a.o_part + at * HD + 4 * c);
+                    y[k] = load_pair(a.o_part + at * HD + 4 * c + 2);
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (q + k * jw < a.parts) join_part(M, L, o, ml[k].x, ml[k].y, (f32x4){x[k].x, x[k].y, y[k].x, y[k].y});
+            }
+        }
+        if (jw > 1) {
+            f32x4* so = (f32x4*)lds;                     // [SLOTS][LPR], then (M, L) of each slot
+            float2* sl = (float2*)(lds + 1024);
+            __syncthreads();
+            so[threadIdx.x] = o;
+            if (c == 0) sl[slot] = make_float2(M, L);
+            __syncthreads();
+            if (w == 0)
+                for (int k = 1; k < jw; ++k) join_part(M, L, o, sl[slot + k].x, sl[slot + k].y, so[threadIdx.x + k * LPR]);
+        }
+        if (on && w == 0) store_row_quad(a.out + (size_t)token * a.ldo + head * HD + 4 * c, L, o);
+    }
+}
 
 // ---- few query rows per group (decode, drafted tokens, a shared prefix): bound by the bytes of the cache.
 // Workgroup = (group, block of 16 MT rows, key range); its 4 waves take the range's tiles in turn, each with a running softmax of its own,
@@ -327,7 +443,7 @@ SEEDMI_DEVINL void lds_fence() { asm volatile("" ::: "memory"); }        // (a w
 // lane's scores are keys 4 g + r of its query li, which is the layout the P^T operand of O^T = V^T P^T needs: P never leaves registers.
 // V is transposed through 8 KiB of LDS that the wave has to itself (no barrier in the loop).
 template <int HD, bool MX, int MT>
-__global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_kernel(const AttnArgs a) {
     constexpr int NT = HD / 16, KS = HD / 32;
     constexpr int VBYTES = KT * HD * 2;
     __shared__ __attribute__((aligned(16))) char sm[4 * (VBYTES > 16 * HD * 4 ? VBYTES : 16 * HD * 4)];
@@ -335,25 +451,27 @@ __global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // eight items (XCDs) side by side, the row blocks of an item behind each other on its XCD
-    const unsigned items = (unsigned)a.groups * a.splits;
-    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    unsigned block;
+    const AttnPass p = pass_of(a, block);
+    const unsigned items = (unsigned)p.groups * p.splits;
+    const unsigned blk = block / (8u * p.row_blocks), in = block % (8u * p.row_blocks);
     const unsigned item = blk * 8 + in % 8;
     const int rb = in / 8;
     if (item >= items) return;
-    const int split = item / a.groups, group = item % a.groups;
-    const int G = a.c.G, slot = group / G, kvh = group % G;
-    const int base = a.shared ? 0 : slot * a.T;          // first token row of the group
-    const int r0 = rb * 16 * MT, r_end = min(a.group_rows, r0 + 16 * MT);
+    const int split = item / p.groups, group = item % p.groups;
+    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int base = p.shared ? 0 : slot * a.T;          // first token row of the group
+    const int r0 = rb * 16 * MT, r_end = min(p.group_rows, r0 + 16 * MT);
 
-    int len = a.kv_len;
-    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
-    len = max(0, min(len, a.c.rows));
-    const bool causal = a.causal && !a.shared;
+    int len = p.kv_len;
+    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
+    len = max(0, min(len, p.c.rows));
+    const bool causal = a.causal && !p.shared;
     // rows of keys that a query row sees: all, or up to its own
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? max(0, min(len, len - a.T + r0 / a.GH + 1)) : len;
     const int tiles = (n_max + KT - 1) / KT;
-    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
     const int t_begin = split * per, t_end = min(tiles, t_begin + per);
 
     bf16x8 qf[MT][KS];
@@ -378,15 +496,16 @@ __global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     constexpr int RB = MX ? HD : 2 * HD;
-    const char* kb = a.c.k + row0 * RB;
-    const char* vb = a.c.v + row0 * RB;
-    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    const char* kb = p.c.k + row0 * RB;
+    const char* vb = p.c.v + row0 * RB;
+    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
     char* lds = sm + wave * VBYTES;
 
     const int last = n_max - 1;
+    arrived(qf);
     Tile<HD, MX> t;
     if (t_begin + wave < t_end) {
         load_v(t, vb, vsb, (t_begin + wave) * KT, last, lane);
@@ -449,15 +568,15 @@ __global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs
                 m[u] = mn;
             }
             const float ref = mn == -INFINITY ? 0.f : mn;
-            float p[2][4];
+            float e[2][4];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
-                    l[u] += p[kt][r];
+                    e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
+                    l[u] += e[kt][r];
                 }
-            pf[u] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0][0], p[0][1]), pack2bf(p[0][2], p[0][3]), pack2bf(p[1][0], p[1][1]), pack2bf(p[1][2], p[1][3])));
+            pf[u] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0][0], e[0][1]), pack2bf(e[0][2], e[0][3]), pack2bf(e[1][0], e[1][1]), pack2bf(e[1][2], e[1][3])));
         }
         if (mixed) {
             // Values that are not finite in a tile that some rows do not see whole: 0 * inf must not reach a row that does not see the key.
@@ -534,16 +653,21 @@ __global__ __launch_bounds__(256, 2) void kv_attention_few_kernel(const AttnArgs
 #pragma unroll
                     for (int d = 0; d < 4; ++d) v[d] += x[d];
                 }
-                if (a.out) {
+                if (a.parts == 1) {
                     const float inv = L == 0.f ? 0.f : 1.f / L;
                     *(uint2*)(a.out + (size_t)token * a.ldo + head * HD + 4 * quad) = make_uint2(pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv));
                 } else {
-                    const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
-                    if (L != 0.f) *(f32x4*)(a.o_part + at * HD + 4 * quad) = v;
-                    if (part == 0 && i == 0) a.ml_part[at] = make_float2(Mr, L);
+                    const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
+                    if (L != 0.f) store_quad(a.o_part + at * HD + 4 * quad, v, a.arrivals != nullptr);
+                    if (part == 0 && i == 0) store_pair((float*)(a.ml_part + at), Mr, L, a.arrivals != nullptr);
                 }
             }
         }
+    }
+    if (a.arrivals) {
+        const int unit = a.unit_rows ? kvh : group * p.row_blocks + rb;
+        const int first = a.unit_rows ? 0 : r0, n_rows = a.unit_rows ? a.unit_rows : r_end - r0;
+        join_in_place<HD>(a, unit, a.unit_rows ? 0 : base, kvh, first, n_rows, (float*)sm);
     }
 }
 
@@ -603,23 +727,25 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     __shared__ __attribute__((aligned(16))) char sm[4 * TB];             // K0 K1 V0 V1
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned items = (unsigned)a.groups * a.splits;
-    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    unsigned block;
+    const AttnPass p = pass_of(a, block);
+    const unsigned items = (unsigned)p.groups * p.splits;
+    const unsigned blk = block / (8u * p.row_blocks), in = block % (8u * p.row_blocks);
     const unsigned item = blk * 8 + in % 8;
-    const int rb = a.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
+    const int rb = p.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
     if (item >= items) return;
-    const int split = item / a.groups, group = item % a.groups;
-    const int G = a.c.G, slot = group / G, kvh = group % G;
-    const int base = a.shared ? 0 : slot * a.T;
-    const int r0 = rb * 64 * MT, r_end = min(a.group_rows, r0 + 64 * MT);
+    const int split = item / p.groups, group = item % p.groups;
+    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int base = p.shared ? 0 : slot * a.T;
+    const int r0 = rb * 64 * MT, r_end = min(p.group_rows, r0 + 64 * MT);
 
-    int len = a.kv_len;
-    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
-    len = max(0, min(len, a.c.rows));
-    const bool causal = a.causal && !a.shared;
+    int len = p.kv_len;
+    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
+    len = max(0, min(len, p.c.rows));
+    const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
-    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
     const int t_begin = split * per, t_end = min(tiles, t_begin + per);
     // what the rows of this wave see at least and at most (its rows may lie beyond the group's end)
     const int w0 = r0 + 16 * MT * wave, w1 = min(r_end - 1, w0 + 16 * MT - 1);
@@ -647,14 +773,15 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = Stage<HD, MX>;
-    const char* kb = a.c.k + row0 * S::RB;
-    const char* vb = a.c.v + row0 * S::RB;
-    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    const char* kb = p.c.k + row0 * S::RB;
+    const char* vb = p.c.v + row0 * S::RB;
+    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
     const int last = n_max - 1;
 
+    arrived(qf);
     S st;
     if (t_begin < t_end) {
         stage_load(st, kb, ksb, vb, vsb, t_begin * KT2, last, tid);
@@ -725,13 +852,13 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
                 const float ref = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
-                    float p[8];
+                    float e[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        p[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
-                        l[u] += p[j];
+                        e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                        l[u] += e[j];
                     }
-                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])));
+                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
                 }
             }
         }
@@ -777,14 +904,14 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
         const int r = w0 + 16 * u + li;
         if (r >= r_end) continue;
         const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
-        if (a.out) {
+        if (a.parts == 1) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 *(uint2*)(op + 16 * n) = make_uint2(pack2bf(o[u][n][0] * inv, o[u][n][1] * inv), pack2bf(o[u][n][2] * inv, o[u][n][3] * inv));
         } else {
-            const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
+            const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
             if (L != 0.f) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) *(f32x4*)(a.o_part + at * HD + 16 * n + 4 * g4) = o[u][n];
@@ -819,24 +946,26 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     __shared__ int s_bad;                                // a tile that some row does not see whole held a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, ht = tid & 255;
-    const unsigned items = (unsigned)a.groups * a.splits;
-    const unsigned blk = blockIdx.x / (8u * a.row_blocks), in = blockIdx.x % (8u * a.row_blocks);
+    unsigned block;
+    const AttnPass p = pass_of(a, block);
+    const unsigned items = (unsigned)p.groups * p.splits;
+    const unsigned blk = block / (8u * p.row_blocks), in = block % (8u * p.row_blocks);
     const unsigned item = blk * 8 + in % 8;
-    const int rb = a.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
+    const int rb = p.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
     if (item >= items) return;
-    const int split = item / a.groups, group = item % a.groups;
-    const int G = a.c.G, slot = group / G, kvh = group % G;
-    const int base = a.shared ? 0 : slot * a.T;
-    const int r0 = rb * 256, r_end = min(a.group_rows, r0 + 256);
+    const int split = item / p.groups, group = item % p.groups;
+    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int base = p.shared ? 0 : slot * a.T;
+    const int r0 = rb * 256, r_end = min(p.group_rows, r0 + 256);
 
-    int len = a.kv_len;
-    if (!a.shared && a.kv_lens) len = a.kv_lens[slot];
-    len = max(0, min(len, a.c.rows));
-    const bool causal = a.causal && !a.shared;
+    int len = p.kv_len;
+    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
+    len = max(0, min(len, p.c.rows));
+    const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? len - a.T + r0 / a.GH + 1 : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
-    const int per = max((tiles + a.splits - 1) / a.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
     const int t0 = split * per, n = max(0, min(tiles, t0 + per) - t0);   // first tile, number of tiles
     const int w0 = r0 + 32 * wave, w1 = min(r_end - 1, w0 + 31);
     const int wave_max = w0 >= r_end ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
@@ -863,16 +992,17 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[u][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const long long row0 = (a.shared ? 0ll : (long long)slot * a.c.slot_rows) + (long long)kvh * a.c.head_rows;
+    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = HalfStage<HD, MX>;
-    const char* kb = a.c.k + row0 * S::RB;
-    const char* vb = a.c.v + row0 * S::RB;
-    const uint8_t* ksb = MX ? a.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? a.c.vs + row0 * (HD / 32) : nullptr;
+    const char* kb = p.c.k + row0 * S::RB;
+    const char* vb = p.c.v + row0 * S::RB;
+    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
+    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
     const int last = n_max - 1;
     const int srow = 32 * half + ht / S::LPR, schunk = ht % S::LPR;      // the thread's first row of a tile and its 16-byte piece of it
     const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
 
+    arrived(qf);
     S st;
     auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const char* b, const uint8_t* sb, int t) {
         if (!stages) return;
@@ -1023,10 +1153,10 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 const float ref = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
-                    float p[8];
+                    float e[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
-                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(p[0], p[1]), pack2bf(p[2], p[3]), pack2bf(p[4], p[5]), pack2bf(p[6], p[7])));
+                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
                 }
             }
         }
@@ -1041,14 +1171,14 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         const int r = w0 + 16 * u + li;
         if (r >= r_end) continue;
         const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
-        if (a.out) {
+        if (a.parts == 1) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
                 *(uint2*)(op + 16 * i) = make_uint2(pack2bf(o[u][i][0] * inv, o[u][i][1] * inv), pack2bf(o[u][i][2] * inv, o[u][i][3] * inv));
         } else {
-            const long long at = (long long)(a.part0 + split) * a.rows + (long long)token * a.H + head;
+            const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
             if (L != 0.f) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) *(f32x4*)(a.o_part + at * HD + 16 * i + 4 * g4) = o[u][i];
@@ -1073,14 +1203,7 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __r
 #pragma unroll 4
         for (int p = w; p < parts; p += JW) {
             const float2 x = ml[p * rows + row];
-            if (x.y == 0.f) continue;                    // nothing there (a NaN sum is not skipped)
-            const f32x4 v = *(const f32x4*)(o_part + (p * rows + row) * HD + 4 * c);
-            const float mn = fmaxf(M, x.x);
-            const float f0 = exp2_hw(M - mn), f1 = exp2_hw(x.x - mn);
-            M = mn;
-            L = L * f0 + x.y * f1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
+            if (x.y != 0.f) join_part(M, L, o, x.x, x.y, *(const f32x4*)(o_part + (p * rows + row) * HD + 4 * c));
         }
     }
     if (JW > 1) {
@@ -1091,22 +1214,13 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __r
         __syncthreads();
         if (w || !on) return;
 #pragma unroll
-        for (int k = 1; k < JW; ++k) {
-            const float2 x = sl[threadIdx.x + k * LPR];
-            if (x.y == 0.f) continue;
-            const f32x4 v = so[threadIdx.x + k * LPR];
-            const float mn = fmaxf(M, x.x);
-            const float f0 = exp2_hw(M - mn), f1 = exp2_hw(x.x - mn);
-            M = mn;
-            L = L * f0 + x.y * f1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
-        }
+        for (int k = 1; k < JW; ++k) join_part(M, L, o, sl[threadIdx.x + k * LPR].x, sl[threadIdx.x + k * LPR].y, so[threadIdx.x + k * LPR]);
     }
-    if (!on) return;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int token = (int)(row / H), head = (int)(row % H);
-    *(uint2*)(out + (size_t)token * ldo + head * HD + 4 * c) = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
+    if (on) store_row_quad(out + (size_t)(row / H) * ldo + (row % H) * HD + 4 * c, L, o);
+}
+
+__global__ void kv_zero_kernel(unsigned* p, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0u;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1214,8 +1328,15 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
 }
 
 // How a call is cut: a pass over the slots' own rows and, with a prefix, one over the prefix; row blocks and key ranges of each.
-struct KvPass { int groups, group_rows, block_rows, row_blocks, splits; };
-struct KvPlan { KvPass own, pre; int parts; long long rows; size_t bytes; };
+struct KvPass { int groups, group_rows, block_rows, row_blocks, splits; unsigned blocks; };
+struct KvPlan {
+    KvPass own, pre;
+    int parts, units, unit_rows;                         // units > 0: joined in place, by the last workgroup of each unit
+    unsigned unit_blocks;
+    long long rows;
+    size_t bytes, o_at;                                  // workspace: arrival counters, (m, l) from KV_WS_COUNTERS on, sums from o_at on
+};
+constexpr size_t KV_WS_COUNTERS = 4096;                  // bytes: 1024 counters
 
 static KvPass plan_pass(int groups, long long rows, long long keys) {
     KvPass p = {};
@@ -1230,6 +1351,7 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);
+    p.blocks = ((unsigned)p.groups * p.splits + 7) / 8 * 8 * p.row_blocks;
     return p;
 }
 
@@ -1246,7 +1368,20 @@ static int make_plan(const seedmi_kv_cache_t* c, int B, int T, int H, int kv_max
     pl->own = plan_pass(B * c->kv_heads, (long long)T * GH, keys);
     pl->pre = prefix_len ? plan_pass(c->kv_heads, (long long)B * T * GH, prefix_len) : KvPass{};
     pl->parts = pl->own.splits + pl->pre.splits;
-    pl->bytes = pl->parts == 1 ? 0 : (((size_t)pl->parts * pl->rows * 8 + 255) & ~(size_t)255) + (size_t)pl->parts * pl->rows * c->head_dim * 4;
+    pl->units = pl->unit_rows = 0;
+    pl->unit_blocks = 0;
+    if (pl->parts > 1 && pl->own.block_rows <= 32 && (!prefix_len || pl->pre.block_rows == pl->own.block_rows)) {
+        // Joined in place where a unit's rows and parts are few enough for one workgroup: a second launch costs about 4 us
+        const int rows = prefix_len ? pl->pre.group_rows : pl->own.block_rows < pl->own.group_rows ? pl->own.block_rows : pl->own.group_rows;
+        const long long units = prefix_len ? c->kv_heads : (long long)pl->own.groups * pl->own.row_blocks;
+        if ((long long)rows * pl->parts <= 64 && units * 4 <= (long long)KV_WS_COUNTERS) {
+            pl->units = (int)units;
+            pl->unit_rows = prefix_len ? rows : 0;
+            pl->unit_blocks = prefix_len ? (unsigned)(pl->pre.row_blocks * pl->pre.splits + B * pl->own.row_blocks * pl->own.splits) : (unsigned)pl->own.splits;
+        }
+    }
+    pl->o_at = (KV_WS_COUNTERS + (size_t)pl->parts * pl->rows * 8 + 255) & ~(size_t)255;
+    pl->bytes = pl->parts == 1 ? 0 : pl->o_at + (size_t)pl->parts * pl->rows * c->head_dim * 4;
     return 0;
 }
 
@@ -1255,41 +1390,58 @@ extern "C" size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* c
     return make_plan(cache, B, T, H, kv_max, prefix_len, &pl) ? 0 : pl.bytes;
 }
 
+extern "C" int seedmi_kv_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
+    if (workspace_bytes == 0) return SEEDMI_OK;
+    if (!workspace || workspace_bytes < KV_WS_COUNTERS || ((uintptr_t)workspace & 255)) {
+        seedmi_set_error("seedmi_kv_attention_workspace_init: need seedmi_kv_attention_workspace_bytes() bytes, 256-byte aligned");
+        return SEEDMI_E_ALIGN;
+    }
+    hipLaunchKernelGGL(kv_zero_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (unsigned*)workspace, (int)(KV_WS_COUNTERS / 4));
+    return seedmi_check_launch("kv_attention_workspace_init");
+}
+
 template <int HD, bool MX>
-static void launch_pass(const AttnArgs& a, const KvPass& p, hipStream_t s) {
-    const unsigned items = (unsigned)p.groups * p.splits;
-    const dim3 grid((items + 7) / 8 * 8 * p.row_blocks);
-    switch (p.block_rows) {
-        case 16: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
-        case 32: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 1>), grid, dim3(256), 0, s, a); break;
-        case 128: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 2>), grid, dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((kv_attention_phased_kernel<HD, MX>), grid, dim3(512), 0, s, a); break;
+static void launch_blocks(const AttnArgs& a, int block_rows, unsigned blocks, hipStream_t s) {
+    switch (block_rows) {
+        case 16: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 1>), dim3(blocks), dim3(256), 0, s, a); break;
+        case 32: hipLaunchKernelGGL((kv_attention_few_kernel<HD, MX, 2>), dim3(blocks), dim3(256), 0, s, a); break;
+        case 64: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 1>), dim3(blocks), dim3(256), 0, s, a); break;
+        case 128: hipLaunchKernelGGL((kv_attention_many_kernel<HD, MX, 2>), dim3(blocks), dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((kv_attention_phased_kernel<HD, MX>), dim3(blocks), dim3(512), 0, s, a); break;
     }
 }
 
 template <int HD, int JW>
-static void launch_join(const AttnArgs& a, const KvPlan& pl, bf16_t* out, hipStream_t s) {
+static void launch_join(const AttnArgs& a, const KvPlan& pl, hipStream_t s) {
     constexpr int RPB = 256 / (HD / 4 * JW);
     hipLaunchKernelGGL((kv_attention_join_kernel<HD, JW>), dim3((unsigned)((pl.rows + RPB - 1) / RPB)), dim3(256), 0, s, a.o_part, a.ml_part,
-                       pl.rows, pl.parts, a.H, out, a.ldo);
+                       pl.rows, pl.parts, a.H, a.out, a.ldo);
 }
 
 template <int HD, bool MX>
-static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, const KvPlan& pl, int prefix_len, bf16_t* out, hipStream_t s) {
-    a.out = pl.parts == 1 ? out : nullptr;
-    auto pass = [&](const KvView& v, const KvPass& p, int shared, int part0) {
-        AttnArgs x = a;
-        x.c = v;
-        x.groups = p.groups; x.group_rows = p.group_rows; x.row_blocks = p.row_blocks; x.splits = p.splits;
-        x.shared = shared; x.part0 = part0;
-        if (shared) { x.kv_len = prefix_len; x.kv_lens = nullptr; }
-        launch_pass<HD, MX>(x, p, s);
+static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, const KvPlan& pl, int prefix_len, int kv_len, const int* kv_lens,
+                             hipStream_t s) {
+    auto set = [](AttnPass& x, const KvView& v, const KvPass& p, int shared, int part0, int len, const int* lens) {
+        x = {v, lens, len, shared, p.groups, p.group_rows, p.row_blocks, p.splits, part0, p.blocks};
     };
-    if (prefix_len) pass(pre, pl.pre, 1, 0);
-    pass(own, pl.own, 0, pl.pre.splits);
-    if (pl.parts > 4) launch_join<HD, 8>(a, pl, out, s);
-    else if (pl.parts > 1) launch_join<HD, 1>(a, pl, out, s);
+    if (!prefix_len) {
+        set(a.pass[0], own, pl.own, 0, 0, kv_len, kv_lens);
+        launch_blocks<HD, MX>(a, pl.own.block_rows, pl.own.blocks, s);
+    } else {
+        set(a.pass[0], pre, pl.pre, 1, 0, prefix_len, nullptr);
+        set(a.pass[1], own, pl.own, 0, pl.pre.splits, kv_len, kv_lens);
+        if (pl.pre.block_rows == pl.own.block_rows) {    // one kernel for both: one launch
+            launch_blocks<HD, MX>(a, pl.own.block_rows, pl.pre.blocks + pl.own.blocks, s);
+        } else {
+            launch_blocks<HD, MX>(a, pl.pre.block_rows, pl.pre.blocks, s);
+            a.pass[0] = a.pass[1];
+            launch_blocks<HD, MX>(a, pl.own.block_rows, pl.own.blocks, s);
+        }
+    }
+    if (pl.parts > 1 && !pl.units) {
+        if (pl.parts > 4) launch_join<HD, 8>(a, pl, s);
+        else launch_join<HD, 1>(a, pl, s);
+    }
 }
 
 extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq,
@@ -1336,13 +1488,15 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
     }
     AttnArgs a = {};
     a.q = (const bf16_t*)q;
+    a.out = (bf16_t*)out;
     a.ldq = ldq; a.ldo = ldo; a.T = T; a.H = H; a.GH = H / G;
-    a.kv_len = kv_len; a.kv_lens = (const int*)kv_lens_i32;
     a.causal = causal; a.c2 = scale * 1.44269504088896340736f;
-    a.rows = pl.rows;
-    a.ml_part = (float2*)workspace;
-    a.o_part = (float*)((char*)workspace + (((size_t)pl.parts * pl.rows * 8 + 255) & ~(size_t)255));
-#define CALL(HD, MX) launch_attention<HD, MX>(a, own, pre, pl, prefix_len, (bf16_t*)out, (hipStream_t)stream)
+    a.rows = pl.rows; a.parts = pl.parts;
+    a.arrivals = pl.units ? (unsigned*)workspace : nullptr;
+    a.unit_blocks = pl.unit_blocks; a.unit_rows = pl.unit_rows;
+    a.ml_part = (float2*)((char*)workspace + KV_WS_COUNTERS);
+    a.o_part = (float*)((char*)workspace + pl.o_at);
+#define CALL(HD, MX) launch_attention<HD, MX>(a, own, pre, pl, prefix_len, kv_len, (const int*)kv_lens_i32, (hipStream_t)stream)
     KV_DISPATCH(hd, cache->format == SEEDMI_KV_MX8, CALL);
 #undef CALL
     return seedmi_check_launch("kv_attention");

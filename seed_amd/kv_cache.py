@@ -22,24 +22,24 @@ _FORMATS = {"16": L.KV_16BIT, "mx8": L.KV_MX8}
 Lengths = Union[int, torch.Tensor]
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# the raw stream of a device's current stream, without the Stream object around it (a decode step pays for every microsecond on the host)
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _On:
-    """The library launches on the current device: the cache's, whatever the caller's is."""
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+def _call(index, fn, name, lib, *args):
+    """One library call on the current stream of device ``index``; the library launches on the current device, so that is switched to it
+    for the call where the caller's is another."""
+    prev = torch.cuda.current_device()
+    if prev == index:
+        rc = fn(*args, _current_stream(index))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(*args, _current_stream(index))
+        finally:
+            torch.cuda.set_device(prev)
+    if rc:
+        L.check(rc, name, lib)
 
 
 class KVCache:
@@ -82,7 +82,8 @@ class KVCache:
         p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         self.struct = L.KVCacheStruct(p(k), p(v), p(k_scale), p(v_scale), slot_rows, head_rows, slots, rows, heads, dim, _FORMATS[fmt])
         self._ref = C.byref(self.struct)
-        self._on = _On(self.device.index)
+        self.index = self.device.index
+        self._append, self._read = self.lib.seedmi_kv_append, self.lib.seedmi_kv_read
 
     @staticmethod
     def _row_strides(t, dim):
@@ -123,15 +124,18 @@ class KVCache:
     def _lengths(self, what: str, n: Lengths, batch: int):
         """(host value, device pointer) of one length for all slots or of an int32 tensor with one each."""
         if isinstance(n, torch.Tensor):
-            if n.dtype != torch.int32 or n.device != self.device or n.numel() < batch or not n.is_contiguous():
+            if n.dtype is not torch.int32 or n.get_device() != self.index or n.numel() < batch or not n.is_contiguous():
                 raise ValueError(f"{what}: lengths must be a contiguous int32 tensor with one entry per slot on {self.device}")
             return 0, n.data_ptr()
         return int(n), None
 
     def _rows_of(self, what: str, x: torch.Tensor, cols: int):
-        if x.dim() != 2 or x.dtype != self.dtype or x.device != self.device or x.shape[1] != cols or x.stride(1) != 1 or x.shape[0] < 1:
-            raise ValueError(f"{what}: expected {self.dtype} rows of {cols} on {self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-        return x.stride(0) if x.shape[0] > 1 else cols
+        """Row stride of x [rows, cols] in the cache's type on its device."""
+        if x.dtype is self.dtype and x.get_device() == self.index and x.dim() == 2 and x.size(1) == cols and x.size(0) > 0:
+            ld, one = x.stride()
+            if one == 1:
+                return ld if x.size(0) > 1 else cols
+        raise ValueError(f"{what}: expected {self.dtype} rows of {cols} on {self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
 
     def _batch(self, what: str, rows: int, lens: Lengths, tokens: Optional[int]):
         """Slots of a call: ``rows`` query rows are ``tokens`` of each, by default of every slot that ``lens`` lists (or of all)."""
@@ -153,23 +157,22 @@ class KVCache:
         ld = self._rows_of("KVCache.append", qkv, (heads + 2 * self.kv_heads) * D)
         B, T = self._batch("KVCache.append", qkv.shape[0], past, tokens)
         n, lens = self._lengths("KVCache.append", past, B)
-        for t in (cos, sin):
-            if t.dtype != self.dtype or t.device != self.device or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != D or not t.is_contiguous():
-                raise ValueError(f"KVCache.append: cos / sin must be contiguous {self.dtype} [positions, {D}] on {self.device}")
-        if pos_ids is not None and (pos_ids.dtype != torch.int64 or pos_ids.device != self.device or pos_ids.numel() != B * T or
-                                    not pos_ids.is_contiguous()):
-            raise ValueError(f"KVCache.append: pos_ids must be {B * T} contiguous int64 on {self.device}")
+        if not (cos.dtype is self.dtype and sin.dtype is self.dtype and cos.get_device() == self.index and sin.get_device() == self.index and
+                cos.dim() == 2 and cos.shape == sin.shape and cos.size(1) == D and cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"KVCache.append: cos / sin must be contiguous {self.dtype} [positions, {D}] on {self.device}")
+        pos = None
+        if pos_ids is not None:
+            if pos_ids.dtype is not torch.int64 or pos_ids.get_device() != self.index or pos_ids.numel() != B * T or not pos_ids.is_contiguous():
+                raise ValueError(f"KVCache.append: pos_ids must be {B * T} contiguous int64 on {self.device}")
+            pos = pos_ids.data_ptr()
         if q_out is None:
-            q_out = torch.empty(B * T, heads * D, dtype=self.dtype, device=self.device)
-        ldq = self._rows_of("KVCache.append (q_out)", q_out, heads * D)
-        if q_out.shape[0] != B * T:
-            raise ValueError(f"KVCache.append: q_out has {q_out.shape[0]} rows, not {B * T}")
-        with self._on:
-            rc = self.lib.seedmi_kv_append(self._ref, qkv.data_ptr(), ld, None if pos_ids is None else pos_ids.data_ptr(), pos_base,
-                                           cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out.data_ptr(), ldq, B, T, heads, n, lens,
-                                           _stream(self.device))
-        if rc:
-            L.check(rc, "seedmi_kv_append", self.lib)
+            q_out, ldq = torch.empty((B * T, heads * D), dtype=self.dtype, device=self.device), heads * D
+        else:
+            ldq = self._rows_of("KVCache.append (q_out)", q_out, heads * D)
+            if q_out.size(0) != B * T:
+                raise ValueError(f"KVCache.append: q_out has {q_out.size(0)} rows, not {B * T}")
+        _call(self.index, self._append, "seedmi_kv_append", self.lib, self._ref, qkv.data_ptr(), ld, pos, pos_base, cos.data_ptr(), sin.data_ptr(),
+              cos.size(0), q_out.data_ptr(), ldq, B, T, heads, n, lens)
         return q_out
 
     def read(self, start: Lengths, n: int, *, slots: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
@@ -181,14 +184,14 @@ class KVCache:
             raise ValueError(f"KVCache.read: {n} rows of {B} of {self.slots} slots")
         at, starts = self._lengths("KVCache.read", start, B)
         shape = (B, self.kv_heads, n, self.head_dim)
-        k_out, v_out = (torch.empty(shape, dtype=self.dtype, device=self.device) if t is None else t for t in (k_out, v_out))
         for t in (k_out, v_out):
-            if tuple(t.shape) != shape or t.dtype != self.dtype or t.device != self.device or not t.is_contiguous():
+            if t is not None and (tuple(t.shape) != shape or t.dtype is not self.dtype or t.get_device() != self.index or not t.is_contiguous()):
                 raise ValueError(f"KVCache.read: outputs must be contiguous {self.dtype} {shape} on {self.device}")
-        with self._on:
-            rc = self.lib.seedmi_kv_read(self._ref, k_out.data_ptr(), v_out.data_ptr(), B, n, at, starts, _stream(self.device))
-        if rc:
-            L.check(rc, "seedmi_kv_read", self.lib)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        _call(self.index, self._read, "seedmi_kv_read", self.lib, self._ref, k_out.data_ptr(), v_out.data_ptr(), B, n, at, starts)
         return k_out, v_out
 
 
@@ -216,26 +219,26 @@ class KVAttention:
         self._pref = self.prefix._ref if self.prefix_len else None
         need = cache.lib.seedmi_kv_attention_workspace_bytes(cache._ref, self.slots, tokens, heads, self.kv_max, self.prefix_len)
         self.workspace = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        if need:
+            _call(cache.index, cache.lib.seedmi_kv_attention_workspace_init, "seedmi_kv_attention_workspace_init", cache.lib,
+                  self.workspace.data_ptr(), need)
         self._ws = (self.workspace.data_ptr(), need) if need else (None, 0)
+        self._fn, self._rows, self._cols = cache.lib.seedmi_kv_attention, self.slots * tokens, heads * cache.head_dim
 
     def __call__(self, q: torch.Tensor, kv_len: Lengths, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q [slots * tokens, heads * head_dim] -> out of the same shape; ``kv_len``: rows each slot holds, the query rows' own included
         (an int, or an int32 tensor with one entry per slot; 0 for an idle slot).  Queries that see nothing get zeros."""
-        c = self.cache
-        cols = self.heads * c.head_dim
+        c, cols, rows = self.cache, self._cols, self._rows
         ldq = c._rows_of("KVAttention", q, cols)
-        if q.shape[0] != self.slots * self.tokens:
-            raise ValueError(f"KVAttention: {q.shape[0]} query rows, made for {self.slots} slots of {self.tokens}")
+        if q.size(0) != rows:
+            raise ValueError(f"KVAttention: {q.size(0)} query rows, made for {self.slots} slots of {self.tokens}")
         n, lens = c._lengths("KVAttention", kv_len, self.slots)
         if out is None:
-            out = torch.empty(q.shape[0], cols, dtype=c.dtype, device=c.device)
-        ldo = c._rows_of("KVAttention (out)", out, cols)
-        if out.shape[0] != q.shape[0]:
-            raise ValueError(f"KVAttention: out has {out.shape[0]} rows, not {q.shape[0]}")
-        with c._on:
-            rc = c.lib.seedmi_kv_attention(c._ref, self._pref, self.prefix_len, q.data_ptr(), ldq, out.data_ptr(), ldo, self.slots, self.tokens,
-                                           self.heads, n, lens, self.kv_max, self.scale, self.causal, self._ws[0], self._ws[1],
-                                           _stream(c.device))
-        if rc:
-            L.check(rc, "seedmi_kv_attention", c.lib)
+            out, ldo = torch.empty((rows, cols), dtype=c.dtype, device=c.device), cols
+        else:
+            ldo = c._rows_of("KVAttention (out)", out, cols)
+            if out.size(0) != rows:
+                raise ValueError(f"KVAttention: out has {out.size(0)} rows, not {rows}")
+        _call(c.index, self._fn, "seedmi_kv_attention", c.lib, c._ref, self._pref, self.prefix_len, q.data_ptr(), ldq, out.data_ptr(), ldo, self.slots,
+              self.tokens, self.heads, n, lens, self.kv_max, self.scale, self.causal, self._ws[0], self._ws[1])
         return out

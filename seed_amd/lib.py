@@ -132,6 +132,7 @@ SIGNATURES = {
     "seedmi_kv_append": (_i, [C.POINTER(KVCacheStruct), _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "seedmi_kv_read": (_i, [C.POINTER(KVCacheStruct), _vp, _vp, _i, _i, _i, _vp, _vp]),
     "seedmi_kv_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KVCacheStruct), _i, _i, _i, _i, _i]),
+    "seedmi_kv_attention_workspace_init": (_i, [_vp, C.c_size_t, _vp]),
     "seedmi_kv_attention": (_i, [C.POINTER(KVCacheStruct), C.POINTER(KVCacheStruct), _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _i,
                                  C.c_float, _i, _vp, C.c_size_t, _vp]),
     "seedmi_preprocess_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i]),

@@ -105,6 +105,12 @@ def test_attention_refuses_a_short_workspace():
     assert L.load().seedmi_kv_attention_workspace_bytes(None, 1, 1, 4, 0, 0) == 0
 
 
+def test_workspace_init_refuses():
+    init = L.load().seedmi_kv_attention_workspace_init
+    assert init(None, 0, None) == 0
+    assert init(None, 8192, None) == E_ALIGN and init(FAKE, 4095, None) == E_ALIGN and init(FAKE + 128, 8192, None) == E_ALIGN
+
+
 def test_layout_of_the_handle(tmp_path):
     """The struct of include/seedmi.h, compiled as plain C, against its ctypes mirror."""
     fields = [f for f, _ in L.KVCacheStruct._fields_]
