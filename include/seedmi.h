@@ -281,7 +281,7 @@ int seedmi_gemm_skinny_packed_bf16(int M, int N, int K, const void* A, int lda, 
 #define SEEDMI_KV_MX8 1            /* rows of head_dim e4m3 bytes + one power-of-two scale byte per 32 of them (1.03 bytes a value) */
 /* Keys and values of `slots` conversations, `kv_heads` heads each: row r of head h of slot s starts at element
  * ((s * slot_rows + h * head_rows) + r) * head_dim of k / v and, for MX8, at byte ((s * slot_rows + h * head_rows) + r) * head_dim / 32 of
- * k_scale / v_scale.  Rows 0 .. rows - 1 of every (slot, head) belong to the caller's allocation; nothing outside them is touched.
+ * k_scale / v_scale.  Rows 0 .. rows - 1 (at most 2^22) of every (slot, head) belong to the caller's allocation; nothing outside them is touched.
  * A contiguous [slots][kv_heads][rows][head_dim] cache has head_rows = rows and slot_rows = kv_heads * rows.  head_dim is 64 or 128.
  * k and v are 16-byte aligned, k_scale and v_scale 4-byte aligned (NULL for 16BIT).
  * MX8: a = the largest finite magnitude of a block of 32; e = the smallest integer >= -126 with a <= 448 * 2^e; scale byte = e + 127; an

@@ -252,6 +252,24 @@ SEEDMI_DEVINL bool bad_words(const uint4& w) { return bad_word(w.x) | bad_word(w
 // zeros in place of what is not finite
 SEEDMI_DEVINL uint32_t clean_word(uint32_t w) { return (bad16(w) ? 0u : w & 0xffffu) | (bad16(w >> 16) ? 0u : w & 0xffff0000u); }
 
+// The rows 0 .. n - 1 of a (slot, head) as buffers: a load takes a per-lane offset that never changes and a scalar one for the tile, and
+// rows from n on read as zeros without touching memory.
+struct RowBuffers { __amdgpu_buffer_rsrc_t k, v, ks, vs; };
+template <int HD, bool MX>
+SEEDMI_DEVINL RowBuffers row_buffers(const KvView& c, long long row0, int n) {
+    constexpr int RB = MX ? HD : 2 * HD;
+    RowBuffers b;
+    b.k = __builtin_amdgcn_make_buffer_rsrc(c.k + row0 * RB, 0, n * RB, 0x00020000);
+    b.v = __builtin_amdgcn_make_buffer_rsrc(c.v + row0 * RB, 0, n * RB, 0x00020000);
+    b.ks = __builtin_amdgcn_make_buffer_rsrc(MX ? c.ks + row0 * (HD / 32) : (uint8_t*)c.k, 0, MX ? n * (HD / 32) : 0, 0x00020000);
+    b.vs = __builtin_amdgcn_make_buffer_rsrc(MX ? c.vs + row0 * (HD / 32) : (uint8_t*)c.k, 0, MX ? n * (HD / 32) : 0, 0x00020000);
+    return b;
+}
+SEEDMI_DEVINL uint4 load16(const __amdgpu_buffer_rsrc_t& r, int lane_off, int tile_off) {
+    const seedmi_u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, lane_off, tile_off, 0);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A tile of 32 keys and values as a wave holds it between the load and its use.
 //   K (the MFMA's A operand, rows = keys): lane (li, g) holds its part of rows 16 kt + li.  16-bit rows: k-step ks = values 32 ks + 8 g ..;
 //     8-bit rows: 16 bytes at 64 j + 16 g = k-steps 2 j and 2 j + 1 (the contraction may run in any order that Q's fragments share).
@@ -265,26 +283,25 @@ struct Tile {
 };
 
 template <int HD, bool MX>
-SEEDMI_DEVINL void load_k(Tile<HD, MX>& t, const char* kb, const uint8_t* ksb, int key0, int last, int lane) {
+SEEDMI_DEVINL void load_k(Tile<HD, MX>& t, const RowBuffers& b, int key0, int lane) {
     constexpr int RB = MX ? HD : 2 * HD;                 // bytes of a row
     const int li = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-        const long long row = min(key0 + 16 * kt + li, last);
 #pragma unroll
-        for (int j = 0; j < Tile<HD, MX>::KL; ++j) t.k[kt][j] = *(const uint4*)(kb + row * RB + 64 * j + 16 * g);
-        if (MX) t.ks[kt] = HD == 128 ? *(const uint32_t*)(ksb + row * 4) : (uint32_t)*(const uint16_t*)(ksb + row * 2);
+        for (int j = 0; j < Tile<HD, MX>::KL; ++j) t.k[kt][j] = load16(b.k, li * RB + 16 * g + 16 * kt * RB + 64 * j, key0 * RB);
+        if (MX) t.ks[kt] = HD == 128 ? __builtin_amdgcn_raw_buffer_load_b32(b.ks, li * 4 + 64 * kt, key0 * 4, 0)
+                                     : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b.ks, li * 2 + 32 * kt, key0 * 2, 0);
     }
 }
 template <int HD, bool MX>
-SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const char* vb, const uint8_t* vsb, int key0, int last, int lane) {
+SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const RowBuffers& b, int key0, int lane) {
     constexpr int RB = MX ? HD : 2 * HD;
     constexpr int LPR = RB / 16;                         // lanes of a row
 #pragma unroll
     for (int j = 0; j < Tile<HD, MX>::VL; ++j) {
-        const long long row = min(key0 + j * (64 / LPR) + lane / LPR, last);
-        t.v[j] = *(const uint4*)(vb + row * RB + 16 * (lane % LPR));
-        if (MX) t.vs[j] = vsb[row * (HD / 32) + (lane % LPR) / 2];
+        t.v[j] = load16(b.v, lane * 16 + 1024 * j, key0 * RB);
+        if (MX) t.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(b.vs, (lane / LPR) * (HD / 32) + (lane % LPR) / 2 + j * (64 / LPR) * (HD / 32), key0 * (HD / 32), 0);
     }
 }
 
@@ -293,16 +310,15 @@ SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const char* vb, const uint8_t* vsb, i
 template <int HD>
 SEEDMI_DEVINL int v_chunk(int row, int c) { return row * (2 * HD) + ((c ^ (row & (HD / 8 - 1))) << 4); }
 
-// The value tile into the LDS image.  TAIL: rows from `rows` on become zeros; returns whether this lane saw a value that is not finite.
-template <int HD, bool MX, bool TAIL>
-SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int rows, int lane) {
+// The value tile into the LDS image.  LOOK: returns whether this lane saw a value that is not finite.
+template <int HD, bool MX, bool LOOK>
+SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int lane) {
     constexpr int LPR = (MX ? HD : 2 * HD) / 16;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < Tile<HD, MX>::VL; ++j) {
         const int row = j * (64 / LPR) + lane / LPR, l = lane % LPR;
-        uint4 w = t.v[j];
-        if (TAIL && row >= rows) w = make_uint4(0, 0, 0, 0);
+        const uint4 w = t.v[j];
         const uint32_t src[4] = {w.x, w.y, w.z, w.w};
         if (MX) {
             const float s = mx_scale_f(t.vs[j]);
@@ -311,14 +327,14 @@ SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int rows, int lane)
             for (int d = 0; d < 4; ++d) {
                 o[2 * d] = mx_unpack2<false>(src[d], s);
                 o[2 * d + 1] = mx_unpack2<true>(src[d], s);
-                if (TAIL) bad |= bad_word(o[2 * d]) | bad_word(o[2 * d + 1]);
+                if (LOOK) bad |= bad_word(o[2 * d]) | bad_word(o[2 * d + 1]);
             }
             *(uint4*)(lds + v_chunk<HD>(row, 2 * l)) = make_uint4(o[0], o[1], o[2], o[3]);
             *(uint4*)(lds + v_chunk<HD>(row, 2 * l + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         } else {
 #pragma unroll
             for (int d = 0; d < 4; ++d)
-                if (TAIL) bad |= bad_word(src[d]);
+                if (LOOK) bad |= bad_word(src[d]);
             *(uint4*)(lds + v_chunk<HD>(row, l)) = w;
         }
     }
@@ -465,7 +481,7 @@ __global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_k
 
     int len = p.kv_len;
     if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = max(0, min(len, p.c.rows));
+    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
     const bool causal = a.causal && !p.shared;
     // rows of keys that a query row sees: all, or up to its own
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
@@ -497,30 +513,25 @@ __global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_k
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
-    constexpr int RB = MX ? HD : 2 * HD;
-    const char* kb = p.c.k + row0 * RB;
-    const char* vb = p.c.v + row0 * RB;
-    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
+    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     char* lds = sm + wave * VBYTES;
 
-    const int last = n_max - 1;
     arrived(qf);
     Tile<HD, MX> t;
     if (t_begin + wave < t_end) {
-        load_v(t, vb, vsb, (t_begin + wave) * KT, last, lane);
-        load_k(t, kb, ksb, (t_begin + wave) * KT, last, lane);
+        load_v(t, rows, (t_begin + wave) * KT, lane);
+        load_k(t, rows, (t_begin + wave) * KT, lane);
     }
 #pragma unroll 1
     for (int tile = t_begin + wave; tile < t_end; tile += 4) {
-        const int key0 = tile * KT, next0 = (tile + 4 < t_end ? tile + 4 : tile) * KT;
+        const int key0 = tile * KT, next0 = (tile + 4 < t_end ? tile + 4 : tiles) * KT;    // (behind the last row: nothing is fetched)
         const bool partial = key0 + KT > n_min;          // (wave-uniform) some row of the block does not see all of the tile
         bool mixed = false;
         lds_fence();
-        if (!partial) stage_v<HD, MX, false>(t, lds, KT, lane);
-        else mixed = __any(stage_v<HD, MX, true>(t, lds, n_max - key0, lane));
+        if (!partial) stage_v<HD, MX, false>(t, lds, lane);
+        else mixed = __any(stage_v<HD, MX, true>(t, lds, lane));
         lds_fence();
-        load_v(t, vb, vsb, next0, last, lane);           // the wave's next tile (its last one again at the end: no branch in the loop)
+        load_v(t, rows, next0, lane);                    // the wave's next tile
         f32x4 s[MT][2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
@@ -543,7 +554,7 @@ __global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_k
                 for (int ks = 0; ks < KS; ++ks) s[u][kt] = seedmi_mfma_16x16x32(kf[ks], qf[u][ks], s[u][kt]);
             }
         }
-        load_k(t, kb, ksb, next0, last, lane);
+        load_k(t, rows, next0, lane);
         bf16x8 pf[MT];
 #pragma unroll
         for (int u = 0; u < MT; ++u) {
@@ -686,17 +697,17 @@ struct Stage {                                           // a thread's part of a
     uint32_t ks[L], vs[L];
 };
 template <int HD, bool MX>
-SEEDMI_DEVINL void stage_load(Stage<HD, MX>& t, const char* kb, const uint8_t* ksb, const char* vb, const uint8_t* vsb, int key0, int last, int tid) {
+SEEDMI_DEVINL void stage_load(Stage<HD, MX>& t, const RowBuffers& b, int key0, int tid) {
     using S = Stage<HD, MX>;
+    const int row = tid / S::LPR, c = tid % S::LPR;
 #pragma unroll
     for (int j = 0; j < S::L; ++j) {
-        const long long row = min(key0 + j * (256 / S::LPR) + tid / S::LPR, last);
-        const int c = tid % S::LPR;
-        t.k[j] = *(const uint4*)(kb + row * S::RB + 16 * c);
-        t.v[j] = *(const uint4*)(vb + row * S::RB + 16 * c);
+        const int r = row + j * (256 / S::LPR);
+        t.k[j] = load16(b.k, r * S::RB + 16 * c, key0 * S::RB);
+        t.v[j] = load16(b.v, r * S::RB + 16 * c, key0 * S::RB);
         if (MX) {
-            t.ks[j] = ksb[row * (HD / 32) + c / 2];
-            t.vs[j] = vsb[row * (HD / 32) + c / 2];
+            t.ks[j] = __builtin_amdgcn_raw_buffer_load_b8(b.ks, r * (HD / 32) + c / 2, key0 * (HD / 32), 0);
+            t.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(b.vs, r * (HD / 32) + c / 2, key0 * (HD / 32), 0);
         }
     }
 }
@@ -741,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 
     int len = p.kv_len;
     if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = max(0, min(len, p.c.rows));
+    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
     const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
@@ -775,18 +786,13 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     }
     const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = Stage<HD, MX>;
-    const char* kb = p.c.k + row0 * S::RB;
-    const char* vb = p.c.v + row0 * S::RB;
-    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
-    const int last = n_max - 1;
-
+    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     arrived(qf);
     S st;
     if (t_begin < t_end) {
-        stage_load(st, kb, ksb, vb, vsb, t_begin * KT2, last, tid);
+        stage_load(st, rows, t_begin * KT2, tid);
         stage_store(st, sm, sm + 2 * TB, tid);
-        stage_load(st, kb, ksb, vb, vsb, min(t_begin + 1, t_end - 1) * KT2, last, tid);
+        stage_load(st, rows, (t_begin + 1 < t_end ? t_begin + 1 : tiles) * KT2, tid);
     }
     __syncthreads();
 #pragma unroll 1
@@ -822,7 +828,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
         // the next tile into the other buffer (read last before the barrier that ended the previous tile), the one after it requested
         if (tile + 1 < t_end) {
             stage_store(st, sm + (cur ^ 1) * TB, sm + (2 + (cur ^ 1)) * TB, tid);
-            stage_load(st, kb, ksb, vb, vsb, min(tile + 2, t_end - 1) * KT2, last, tid);
+            stage_load(st, rows, (tile + 2 < t_end ? tile + 2 : tiles) * KT2, tid);
         }
         bf16x8 pf[MT][2];
         if (live) {
@@ -960,7 +966,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 
     int len = p.kv_len;
     if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = max(0, min(len, p.c.rows));
+    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
     const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? len - a.T + r0 / a.GH + 1 : len;
@@ -994,23 +1000,20 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     }
     const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = HalfStage<HD, MX>;
-    const char* kb = p.c.k + row0 * S::RB;
-    const char* vb = p.c.v + row0 * S::RB;
-    const uint8_t* ksb = MX ? p.c.ks + row0 * (HD / 32) : nullptr;
-    const uint8_t* vsb = MX ? p.c.vs + row0 * (HD / 32) : nullptr;
-    const int last = n_max - 1;
+    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     const int srow = 32 * half + ht / S::LPR, schunk = ht % S::LPR;      // the thread's first row of a tile and its 16-byte piece of it
     const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
 
     arrived(qf);
     S st;
-    auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const char* b, const uint8_t* sb, int t) {
+    auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const __amdgpu_buffer_rsrc_t& b, const __amdgpu_buffer_rsrc_t& sb, int t) {
         if (!stages) return;
+        const int key0 = (t < n ? t0 + t : tiles) * KT2;
 #pragma unroll
         for (int j = 0; j < S::L; ++j) {
-            const long long row = min((t0 + min(t, n - 1)) * KT2 + srow + j * (256 / S::LPR), last);
-            w[j] = *(const uint4*)(b + row * S::RB + 16 * schunk);
-            if (MX) sc[j] = sb[row * (HD / 32) + schunk / 2];
+            const int r = srow + j * (256 / S::LPR);
+            w[j] = load16(b, r * S::RB + 16 * schunk, key0 * S::RB);
+            if (MX) sc[j] = __builtin_amdgcn_raw_buffer_load_b8(sb, r * (HD / 32) + schunk / 2, key0 * (HD / 32), 0);
         }
     };
     // raw: where a value tile that some row does not see whole leaves its rows as they are; the image then holds zeros in place of what is not
@@ -1047,16 +1050,16 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     if (tid == 0) s_bad = 0;
     __syncthreads();
     if (n > 0) {
-        load_rows(st.k, st.ks, kb, ksb, 0);
+        load_rows(st.k, st.ks, rows.k, rows.ks, 0);
         store_rows(st.k, st.ks, kbuf(0), nullptr);
         if (half) {                                      // half 1 is one vector phase ahead in its staging
-            load_rows(st.k, st.ks, kb, ksb, 1);
-            load_rows(st.v, st.vs, vb, vsb, 0);
+            load_rows(st.k, st.ks, rows.k, rows.ks, 1);
+            load_rows(st.v, st.vs, rows.v, rows.vs, 0);
             if (n > 1) store_rows(st.k, st.ks, kbuf(1), nullptr);
             store_rows(st.v, st.vs, vbuf(0), vraw(0));
         }
-        load_rows(st.k, st.ks, kb, ksb, 1 + half);
-        load_rows(st.v, st.vs, vb, vsb, half);
+        load_rows(st.k, st.ks, rows.k, rows.ks, 1 + half);
+        load_rows(st.v, st.vs, rows.v, rows.vs, half);
     }
     __syncthreads();
 
@@ -1123,8 +1126,8 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         // ---- vector phase
         if (t + 1 + half < n) store_rows(st.k, st.ks, kbuf(t + 1 + half), nullptr);
         if (t + half < n) store_rows(st.v, st.vs, vbuf(t + half), vraw(t + half));
-        load_rows(st.k, st.ks, kb, ksb, t + 2 + half);
-        load_rows(st.v, st.vs, vb, vsb, t + 1 + half);
+        load_rows(st.k, st.ks, rows.k, rows.ks, t + 2 + half);
+        load_rows(st.v, st.vs, rows.v, rows.vs, t + 1 + half);
         if (live) {
 #pragma unroll
             for (int u = 0; u < MT; ++u) {
@@ -1227,6 +1230,10 @@ __global__ void kv_zero_kernel(unsigned* p, int n) {
 int check_cache(const char* who, const seedmi_kv_cache_t* c, KvView* v) {
     if (!c || !c->k || !c->v || c->slots <= 0 || c->rows <= 0 || c->kv_heads <= 0 || c->head_rows < 0 || c->slot_rows < 0) {
         seedmi_set_error("%s: cache handle: null pointer or slots / rows / kv_heads <= 0 or a negative stride", who);
+        return SEEDMI_E_SHAPE;
+    }
+    if (c->rows > 1 << 22) {                               // (32-bit offsets inside a (slot, head))
+        seedmi_set_error("%s: %d rows (at most 2^22)", who, c->rows);
         return SEEDMI_E_SHAPE;
     }
     if (c->head_dim != 64 && c->head_dim != 128) {
@@ -1347,7 +1354,7 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     const int kt = p.block_rows <= 32 ? KT : KT2;
     const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
-    const long long target = p.block_rows == 16 ? 768 : p.block_rows == 256 ? 256 : 512;              // workgroups that the 256 CUs hold at once
+    const long long target = 256;                                         // one workgroup per CU: more ranges cost more in parts than they balance
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);

@@ -44,6 +44,7 @@ def _attend(h, p=None, **kw):
 
 @pytest.mark.parametrize("call", [_append, _read, _attend])
 @pytest.mark.parametrize("bad,code", [(dict(k=None), E_SHAPE), (dict(slots=0), E_SHAPE), (dict(rows=0), E_SHAPE), (dict(kv_heads=0), E_SHAPE),
+                                      (dict(rows=(1 << 22) + 1), E_SHAPE),
                                       (dict(head_dim=96), E_SHAPE), (dict(format=2), E_DTYPE), (dict(k_scale=None), E_SHAPE),
                                       (dict(format=L.KV_16BIT), E_SHAPE), (dict(v=FAKE + 8), E_ALIGN), (dict(v_scale=FAKE + 2), E_ALIGN),
                                       (dict(head_rows=-1), E_SHAPE), (dict(slot_rows=-64), E_SHAPE)])
