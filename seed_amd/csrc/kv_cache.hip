@@ -305,10 +305,12 @@ SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const RowBuffers& b, int key0, int la
     }
 }
 
-// position of 16-byte chunk c of value row `row` in the LDS image: chunks are XOR-ed with the row, so that both the row-wise writes and the
-// transposing reads (4 rows x 32 bytes per 16 lanes) spread over the banks
+// LDS images of widened tiles: rows of 2 HD bytes, padded so that the rows that are read together lie on different banks (keys: 16 bytes of
+// 16 rows at a time; values: 32 bytes of 8 rows, the transposing read) and every address is a lane's own plus a constant.
 template <int HD>
-SEEDMI_DEVINL int v_chunk(int row, int c) { return row * (2 * HD) + ((c ^ (row & (HD / 8 - 1))) << 4); }
+SEEDMI_DEVINL constexpr int k_at(int row, int c) { return row * (2 * HD + 16) + 16 * c; }                // 16-byte chunk c of a key row
+template <int HD>
+SEEDMI_DEVINL constexpr int v_at(int row, int c) { return row * (2 * HD + 32) + 16 * c; }                // ... of a value row
 
 // The value tile into the LDS image.  LOOK: returns whether this lane saw a value that is not finite.
 template <int HD, bool MX, bool LOOK>
@@ -329,13 +331,13 @@ SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int lane) {
                 o[2 * d + 1] = mx_unpack2<true>(src[d], s);
                 if (LOOK) bad |= bad_word(o[2 * d]) | bad_word(o[2 * d + 1]);
             }
-            *(uint4*)(lds + v_chunk<HD>(row, 2 * l)) = make_uint4(o[0], o[1], o[2], o[3]);
-            *(uint4*)(lds + v_chunk<HD>(row, 2 * l + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+            *(uint4*)(lds + v_at<HD>(row, 2 * l)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *(uint4*)(lds + v_at<HD>(row, 2 * l + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
         } else {
 #pragma unroll
             for (int d = 0; d < 4; ++d)
                 if (LOOK) bad |= bad_word(src[d]);
-            *(uint4*)(lds + v_chunk<HD>(row, l)) = w;
+            *(uint4*)(lds + v_at<HD>(row, l)) = w;
         }
     }
     return bad;
@@ -346,8 +348,8 @@ template <int HD>
 SEEDMI_DEVINL bf16x8 v_frag(const char* lds, int n, int lane) {
     const int li = lane & 15, g = lane >> 4;
     const int row = 4 * g + (li >> 2), c = 2 * n + ((li & 3) >> 1), b8 = (li & 1) << 3;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_chunk<HD>(row, c) + b8));
-    const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_chunk<HD>(row + 16, c) + b8));
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_at<HD>(row, c) + b8));
+    const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + v_at<HD>(row + 16, c) + b8));
     const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, z);
     return __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y));
 }
@@ -459,10 +461,10 @@ SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh,
 // lane's scores are keys 4 g + r of its query li, which is the layout the P^T operand of O^T = V^T P^T needs: P never leaves registers.
 // V is transposed through 8 KiB of LDS that the wave has to itself (no barrier in the loop).
 template <int HD, bool MX, int MT>
-__global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_few_kernel(const AttnArgs a) {
     constexpr int NT = HD / 16, KS = HD / 32;
-    constexpr int VBYTES = KT * HD * 2;
-    __shared__ __attribute__((aligned(16))) char sm[4 * (VBYTES > 16 * HD * 4 ? VBYTES : 16 * HD * 4)];
+    constexpr int VBYTES = v_at<HD>(KT, 0);
+    __shared__ __attribute__((aligned(16))) char sm[4 * VBYTES];               // >= 4 * 16 * HD floats: the join below
     __shared__ float2 sml[4][16];
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -593,11 +595,12 @@ __global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_k
             // Values that are not finite in a tile that some rows do not see whole: 0 * inf must not reach a row that does not see the key.
             // They are added here to the rows that do, and taken out of the image.
             lds_fence();
+            const int ln = fresh_lane(), g = ln >> 4;    // (cold: no address of this block is kept across the loop)
 #pragma unroll 1
             for (int j = 0; j < KT; ++j) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint2 w = *(const uint2*)(lds + v_chunk<HD>(j, 2 * n + (g4 >> 1)) + 8 * (g4 & 1));
+                    const uint2 w = *(const uint2*)(lds + v_at<HD>(j, 2 * n) + 8 * g);
                     const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(256, MX && MT == 1 ? 3 : 2) void kv_attention_few_k
             }
             lds_fence();
 #pragma unroll 1
-            for (int i = 16 * lane; i < VBYTES; i += 1024) {
+            for (int i = 16 * ln; i < VBYTES; i += 1024) {
                 uint32_t* w = (uint32_t*)(lds + i);
 #pragma unroll
                 for (int d = 0; d < 4; ++d) w[d] = clean_word(w[d]);
@@ -714,28 +717,28 @@ SEEDMI_DEVINL void stage_load(Stage<HD, MX>& t, const RowBuffers& b, int key0, i
 template <int HD, bool MX>
 SEEDMI_DEVINL void stage_store(const Stage<HD, MX>& t, char* kl, char* vl, int tid) {
     using S = Stage<HD, MX>;
-    auto put = [](char* dst, uint4 w, uint32_t sb, int row, int c) {
+    auto put = [](char* dst, uint4 w, uint32_t sb) {
         if (MX) {
             const float s = mx_scale_f(sb);
-            *(uint4*)(dst + v_chunk<HD>(row, 2 * c)) = make_uint4(mx_unpack2<false>(w.x, s), mx_unpack2<true>(w.x, s), mx_unpack2<false>(w.y, s), mx_unpack2<true>(w.y, s));
-            *(uint4*)(dst + v_chunk<HD>(row, 2 * c + 1)) = make_uint4(mx_unpack2<false>(w.z, s), mx_unpack2<true>(w.z, s), mx_unpack2<false>(w.w, s), mx_unpack2<true>(w.w, s));
+            *(uint4*)dst = make_uint4(mx_unpack2<false>(w.x, s), mx_unpack2<true>(w.x, s), mx_unpack2<false>(w.y, s), mx_unpack2<true>(w.y, s));
+            *(uint4*)(dst + 16) = make_uint4(mx_unpack2<false>(w.z, s), mx_unpack2<true>(w.z, s), mx_unpack2<false>(w.w, s), mx_unpack2<true>(w.w, s));
         } else {
-            *(uint4*)(dst + v_chunk<HD>(row, c)) = make_uint4(w.x, w.y, w.z, w.w);
+            *(uint4*)dst = make_uint4(w.x, w.y, w.z, w.w);
         }
     };
 #pragma unroll
     for (int j = 0; j < S::L; ++j) {
         const int row = j * (256 / S::LPR) + tid / S::LPR, c = tid % S::LPR;
-        put(kl, t.k[j], MX ? t.ks[j] : 0u, row, c);
-        put(vl, t.v[j], MX ? t.vs[j] : 0u, row, c);
+        put(kl + k_at<HD>(row, MX ? 2 * c : c), t.k[j], MX ? t.ks[j] : 0u);
+        put(vl + v_at<HD>(row, MX ? 2 * c : c), t.v[j], MX ? t.vs[j] : 0u);
     }
 }
 
 template <int HD, bool MX, int MT>
 __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArgs a) {
     constexpr int NT = HD / 16, KS = HD / 32;
-    constexpr int TB = KT2 * HD * 2;                     // bytes of a widened tile
-    __shared__ __attribute__((aligned(16))) char sm[4 * TB];             // K0 K1 V0 V1
+    constexpr int KB = k_at<HD>(KT2, 0), VB = v_at<HD>(KT2, 0);          // bytes of the images
+    __shared__ __attribute__((aligned(16))) char sm[2 * KB + 2 * VB];    // K0 K1 V0 V1
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     unsigned block;
@@ -791,22 +794,20 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     S st;
     if (t_begin < t_end) {
         stage_load(st, rows, t_begin * KT2, tid);
-        stage_store(st, sm, sm + 2 * TB, tid);
+        stage_store(st, sm, sm + 2 * KB, tid);
         stage_load(st, rows, (t_begin + 1 < t_end ? t_begin + 1 : tiles) * KT2, tid);
     }
     __syncthreads();
 #pragma unroll 1
     for (int tile = t_begin; tile < t_end; ++tile) {
         const int key0 = tile * KT2, cur = (tile - t_begin) & 1;
-        char* kl = sm + cur * TB;
-        char* vl = sm + (2 + cur) * TB;
+        char* kl = sm + cur * KB;
+        char* vl = sm + 2 * KB + cur * VB;
         bool mixed = false;
         if (key0 + KT2 > n_max || (causal && key0 + KT2 > len - a.T + r0 / a.GH + 1)) {          // (uniform) some row does not see it all
             bool bad = false;
 #pragma unroll 1
-            for (int i = 4 * tid; i < TB; i += 1024) {
-                bad |= bad_word(*(const uint32_t*)(vl + i));
-            }
+            for (int i = 16 * tid; i < KT2 * 2 * HD; i += 4096) bad |= bad_words(*(const uint4*)(vl + v_at<HD>(i / (2 * HD), i % (2 * HD) / 16)));
             mixed = __syncthreads_or(bad) != 0;
         }
         f32x4 s[MT][4];
@@ -816,7 +817,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             for (int kt = 0; kt < 4; ++kt) {
                 bf16x8 kf[KS];
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + v_chunk<HD>(16 * kt + li, 4 * ks + g4));
+                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + k_at<HD>(16 * kt + li, 4 * ks + g4));
 #pragma unroll
                 for (int u = 0; u < MT; ++u) {
                     s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
         }
         // the next tile into the other buffer (read last before the barrier that ended the previous tile), the one after it requested
         if (tile + 1 < t_end) {
-            stage_store(st, sm + (cur ^ 1) * TB, sm + (2 + (cur ^ 1)) * TB, tid);
+            stage_store(st, sm + (cur ^ 1) * KB, sm + 2 * KB + (cur ^ 1) * VB, tid);
             stage_load(st, rows, (tile + 2 < t_end ? tile + 2 : tiles) * KT2, tid);
         }
         bf16x8 pf[MT][2];
@@ -870,11 +871,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
         }
         if (mixed) {                                     // see kv_attention_few_kernel
             if (live) {
+                const int g = fresh_lane() >> 4;
 #pragma unroll 1
                 for (int j = 0; j < KT2; ++j) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const uint2 w = *(const uint2*)(vl + v_chunk<HD>(j, 2 * n + (g4 >> 1)) + 8 * (g4 & 1));
+                        const uint2 w = *(const uint2*)(vl + v_at<HD>(j, 2 * n) + 8 * g);
                         const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
@@ -886,9 +888,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             }
             __syncthreads();
 #pragma unroll 1
-            for (int i = 4 * tid; i < TB; i += 1024) {
-                *(uint32_t*)(vl + i) = clean_word(*(uint32_t*)(vl + i));
-            }
+            for (int i = 4 * tid; i < VB; i += 1024) *(uint32_t*)(vl + i) = clean_word(*(uint32_t*)(vl + i));
             __syncthreads();
         }
         if (live) {
@@ -896,7 +896,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const bf16x8 vf = v_frag<HD>(vl + kk * (32 * 2 * HD), n, lane);
+                    const bf16x8 vf = v_frag<HD>(vl + v_at<HD>(32 * kk, 0), n, lane);
 #pragma unroll
                     for (int u = 0; u < MT; ++u) o[u][n] = seedmi_mfma_16x16x32(vf, pf[u][kk], o[u][n]);
                 }
@@ -947,8 +947,8 @@ struct HalfStage {                                       // a thread's part of 3
 template <int HD, bool MX>
 __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs a) {
     constexpr int MT = 2, NT = HD / 16, KS = HD / 32;
-    constexpr int TB = KT2 * HD * 2;
-    __shared__ __attribute__((aligned(16))) char sm[6 * TB];             // K0 K1 V0 V1, raw V0 V1
+    constexpr int KB = k_at<HD>(KT2, 0), VB = v_at<HD>(KT2, 0);          // bytes of the images
+    __shared__ __attribute__((aligned(16))) char sm[2 * KB + 4 * VB];    // K0 K1, V0 V1, raw V0 V1
     __shared__ int s_bad;                                // a tile that some row does not see whole held a value that is not finite
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, ht = tid & 255;
@@ -1005,6 +1005,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
 
     arrived(qf);
+    constexpr int KP = k_at<HD>(1, 0), VP = v_at<HD>(1, 0);              // row pitches of the images
     S st;
     auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const __amdgpu_buffer_rsrc_t& b, const __amdgpu_buffer_rsrc_t& sb, int t) {
         if (!stages) return;
@@ -1018,7 +1019,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     };
     // raw: where a value tile that some row does not see whole leaves its rows as they are; the image then holds zeros in place of what is not
     // finite (0 * inf must not reach a row that does not see the key; the rows that do take it from the raw rows)
-    auto store_rows = [&](const uint4 (&w)[S::L], const uint32_t (&sc)[S::L], char* dst, char* raw) {
+    auto store_rows = [&](const uint4 (&w)[S::L], const uint32_t (&sc)[S::L], char* dst, int pitch, char* raw) {
         if (!stages) return;
         bool bad = false;
         auto put = [&](int at, uint4 x) {
@@ -1031,32 +1032,32 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         };
 #pragma unroll
         for (int j = 0; j < S::L; ++j) {
-            const int row = srow + j * (256 / S::LPR);
+            const int at = (srow + j * (256 / S::LPR)) * pitch + (MX ? 32 : 16) * schunk;
             if (MX) {
                 const float s = mx_scale_f(sc[j]);
-                put(v_chunk<HD>(row, 2 * schunk), make_uint4(mx_unpack2<false>(w[j].x, s), mx_unpack2<true>(w[j].x, s), mx_unpack2<false>(w[j].y, s), mx_unpack2<true>(w[j].y, s)));
-                put(v_chunk<HD>(row, 2 * schunk + 1), make_uint4(mx_unpack2<false>(w[j].z, s), mx_unpack2<true>(w[j].z, s), mx_unpack2<false>(w[j].w, s), mx_unpack2<true>(w[j].w, s)));
+                put(at, make_uint4(mx_unpack2<false>(w[j].x, s), mx_unpack2<true>(w[j].x, s), mx_unpack2<false>(w[j].y, s), mx_unpack2<true>(w[j].y, s)));
+                put(at + 16, make_uint4(mx_unpack2<false>(w[j].z, s), mx_unpack2<true>(w[j].z, s), mx_unpack2<false>(w[j].w, s), mx_unpack2<true>(w[j].w, s)));
             } else {
-                put(v_chunk<HD>(row, schunk), make_uint4(w[j].x, w[j].y, w[j].z, w[j].w));
+                put(at, make_uint4(w[j].x, w[j].y, w[j].z, w[j].w));
             }
         }
         if (raw && bad) s_bad = 1;
     };
-    auto kbuf = [&](int t) { return sm + (t & 1) * TB; };
-    auto vbuf = [&](int t) { return sm + (2 + (t & 1)) * TB; };
+    auto kbuf = [&](int t) { return sm + (t & 1) * KB; };
+    auto vbuf = [&](int t) { return sm + 2 * KB + (t & 1) * VB; };
     auto mixed_tile = [&](int t) { return (t0 + t + 1) * KT2 > n_min; }; // some row of the block does not see all of it
-    auto vraw = [&](int t) { return mixed_tile(t) ? sm + (4 + (t & 1)) * TB : nullptr; };
+    auto vraw = [&](int t) { return mixed_tile(t) ? sm + 2 * KB + (2 + (t & 1)) * VB : nullptr; };
 
     if (tid == 0) s_bad = 0;
     __syncthreads();
     if (n > 0) {
         load_rows(st.k, st.ks, rows.k, rows.ks, 0);
-        store_rows(st.k, st.ks, kbuf(0), nullptr);
+        store_rows(st.k, st.ks, kbuf(0), KP, nullptr);
         if (half) {                                      // half 1 is one vector phase ahead in its staging
             load_rows(st.k, st.ks, rows.k, rows.ks, 1);
             load_rows(st.v, st.vs, rows.v, rows.vs, 0);
-            if (n > 1) store_rows(st.k, st.ks, kbuf(1), nullptr);
-            store_rows(st.v, st.vs, vbuf(0), vraw(0));
+            if (n > 1) store_rows(st.k, st.ks, kbuf(1), KP, nullptr);
+            store_rows(st.v, st.vs, vbuf(0), VP, vraw(0));
         }
         load_rows(st.k, st.ks, rows.k, rows.ks, 1 + half);
         load_rows(st.v, st.vs, rows.v, rows.vs, half);
@@ -1071,7 +1072,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const bf16x8 vf = v_frag<HD>(vl + kk * (32 * 2 * HD), i, lane);
+                const bf16x8 vf = v_frag<HD>(vl + v_at<HD>(32 * kk, 0), i, lane);
 #pragma unroll
                 for (int u = 0; u < MT; ++u) o[u][i] = seedmi_mfma_16x16x32(vf, pf[u][kk], o[u][i]);
             }
@@ -1080,12 +1081,13 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 #pragma unroll
             for (int u = 0; u < MT; ++u) l[u] = seedmi_mfma_16x16x32(ones, pf[u][kk], l[u]);
         if (__builtin_expect(mixed_tile(t) && __builtin_amdgcn_readfirstlane(s_bad), 0)) {
-            const char* rl = sm + (4 + (t & 1)) * TB;
+            const int g = fresh_lane() >> 4;
+            const char* rl = sm + 2 * KB + (2 + (t & 1)) * VB;
 #pragma unroll 1
             for (int j = 0; j < KT2; ++j) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const uint2 w = *(const uint2*)(rl + v_chunk<HD>(j, 2 * i + (g4 >> 1)) + 8 * (g4 & 1));
+                    const uint2 w = *(const uint2*)(rl + v_at<HD>(j, 2 * i) + 8 * g);
                     const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -1112,7 +1114,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
             for (int kt = 0; kt < 4; ++kt) {
                 bf16x8 kf[KS];
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + v_chunk<HD>(16 * kt + li, 4 * ks + g4));
+                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + k_at<HD>(16 * kt + li, 4 * ks + g4));
 #pragma unroll
                 for (int u = 0; u < MT; ++u) {
                     s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -1124,8 +1126,8 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         __builtin_amdgcn_s_setprio(0);
         __syncthreads();
         // ---- vector phase
-        if (t + 1 + half < n) store_rows(st.k, st.ks, kbuf(t + 1 + half), nullptr);
-        if (t + half < n) store_rows(st.v, st.vs, vbuf(t + half), vraw(t + half));
+        if (t + 1 + half < n) store_rows(st.k, st.ks, kbuf(t + 1 + half), KP, nullptr);
+        if (t + half < n) store_rows(st.v, st.vs, vbuf(t + half), VP, vraw(t + half));
         load_rows(st.k, st.ks, rows.k, rows.ks, t + 2 + half);
         load_rows(st.v, st.vs, rows.v, rows.vs, t + 1 + half);
         if (live) {
