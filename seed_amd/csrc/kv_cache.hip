@@ -191,7 +191,7 @@ struct AttnPass {                                       // one pass: the slots' 
     const int* kv_lens;
     int kv_len, shared;                                  // shared: the groups are those of the prefix (kv_len rows, all visible)
     int groups, group_rows, row_blocks;                  // groups = slots * G (prefix: G), rows of a group, row blocks of a group
-    int splits, part0;                                   // key ranges and the first one's part index
+    int splits, part0, per_split;                        // key ranges, the first one's part index, tiles of a range (at least)
     unsigned blocks;                                     // workgroups of the pass
 };
 struct AttnArgs {
@@ -214,7 +214,7 @@ SEEDMI_DEVINL AttnPass pass_of(const AttnArgs& a, unsigned& block) {
     AttnPass p;
 #define SEL(f) p.f = second ? a.pass[1].f : a.pass[0].f
     SEL(c.k); SEL(c.v); SEL(c.ks); SEL(c.vs); SEL(c.slot_rows); SEL(c.head_rows); SEL(c.rows); SEL(c.G);
-    SEL(kv_lens); SEL(kv_len); SEL(shared); SEL(groups); SEL(group_rows); SEL(row_blocks); SEL(splits); SEL(part0); SEL(blocks);
+    SEL(kv_lens); SEL(kv_len); SEL(shared); SEL(groups); SEL(group_rows); SEL(row_blocks); SEL(splits); SEL(part0); SEL(per_split); SEL(blocks);
 #undef SEL
     return p;
 }
@@ -270,6 +270,17 @@ SEEDMI_DEVINL uint4 load16(const __amdgpu_buffer_rsrc_t& r, int lane_off, int ti
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Scale bytes of a row, for a lane that needs the one of block `blk`.  Rows of 128 values: the row's four bytes as one word, the byte taken at
+// its use.  (A byte load is widened in the loop's last block by this compiler: a wait for the loads of the next tile, in every iteration.
+// Rows of 64 have two bytes and no word of their own.)
+template <int HD>
+SEEDMI_DEVINL uint32_t load_scale(const __amdgpu_buffer_rsrc_t& r, int row, int blk, int tile_off) {
+    if (HD == 128) return __builtin_amdgcn_raw_buffer_load_b32(r, row * 4, tile_off, 0);
+    return __builtin_amdgcn_raw_buffer_load_b8(r, row * (HD / 32) + blk, tile_off, 0);
+}
+template <int HD>
+SEEDMI_DEVINL float scale_of(uint32_t loaded, int blk) { return mx_scale_f(HD == 128 ? (loaded >> (8 * blk)) & 255u : loaded); }
+
 // A tile of 32 keys and values as a wave holds it between the load and its use.
 //   K (the MFMA's A operand, rows = keys): lane (li, g) holds its part of rows 16 kt + li.  16-bit rows: k-step ks = values 32 ks + 8 g ..;
 //     8-bit rows: 16 bytes at 64 j + 16 g = k-steps 2 j and 2 j + 1 (the contraction may run in any order that Q's fragments share).
@@ -301,7 +312,7 @@ SEEDMI_DEVINL void load_v(Tile<HD, MX>& t, const RowBuffers& b, int key0, int la
 #pragma unroll
     for (int j = 0; j < Tile<HD, MX>::VL; ++j) {
         t.v[j] = load16(b.v, lane * 16 + 1024 * j, key0 * RB);
-        if (MX) t.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(b.vs, (lane / LPR) * (HD / 32) + (lane % LPR) / 2 + j * (64 / LPR) * (HD / 32), key0 * (HD / 32), 0);
+        if (MX) t.vs[j] = load_scale<HD>(b.vs, lane / LPR + j * (64 / LPR), (lane % LPR) / 2, key0 * (HD / 32));
     }
 }
 
@@ -323,7 +334,7 @@ SEEDMI_DEVINL bool stage_v(const Tile<HD, MX>& t, char* lds, int lane) {
         const uint4 w = t.v[j];
         const uint32_t src[4] = {w.x, w.y, w.z, w.w};
         if (MX) {
-            const float s = mx_scale_f(t.vs[j]);
+            const float s = scale_of<HD>(t.vs[j], l / 2);
             uint32_t o[8];
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
@@ -489,7 +500,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? max(0, min(len, len - a.T + r0 / a.GH + 1)) : len;
     const int tiles = (n_max + KT - 1) / KT;
-    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, p.per_split);
     const int t_begin = split * per, t_end = min(tiles, t_begin + per);
 
     bf16x8 qf[MT][KS];
@@ -709,17 +720,17 @@ SEEDMI_DEVINL void stage_load(Stage<HD, MX>& t, const RowBuffers& b, int key0, i
         t.k[j] = load16(b.k, r * S::RB + 16 * c, key0 * S::RB);
         t.v[j] = load16(b.v, r * S::RB + 16 * c, key0 * S::RB);
         if (MX) {
-            t.ks[j] = __builtin_amdgcn_raw_buffer_load_b8(b.ks, r * (HD / 32) + c / 2, key0 * (HD / 32), 0);
-            t.vs[j] = __builtin_amdgcn_raw_buffer_load_b8(b.vs, r * (HD / 32) + c / 2, key0 * (HD / 32), 0);
+            t.ks[j] = load_scale<HD>(b.ks, r, c / 2, key0 * (HD / 32));
+            t.vs[j] = load_scale<HD>(b.vs, r, c / 2, key0 * (HD / 32));
         }
     }
 }
 template <int HD, bool MX>
 SEEDMI_DEVINL void stage_store(const Stage<HD, MX>& t, char* kl, char* vl, int tid) {
     using S = Stage<HD, MX>;
-    auto put = [](char* dst, uint4 w, uint32_t sb) {
+    auto put = [](char* dst, uint4 w, uint32_t sb, int blk) {
         if (MX) {
-            const float s = mx_scale_f(sb);
+            const float s = scale_of<HD>(sb, blk);
             *(uint4*)dst = make_uint4(mx_unpack2<false>(w.x, s), mx_unpack2<true>(w.x, s), mx_unpack2<false>(w.y, s), mx_unpack2<true>(w.y, s));
             *(uint4*)(dst + 16) = make_uint4(mx_unpack2<false>(w.z, s), mx_unpack2<true>(w.z, s), mx_unpack2<false>(w.w, s), mx_unpack2<true>(w.w, s));
         } else {
@@ -729,8 +740,8 @@ SEEDMI_DEVINL void stage_store(const Stage<HD, MX>& t, char* kl, char* vl, int t
 #pragma unroll
     for (int j = 0; j < S::L; ++j) {
         const int row = j * (256 / S::LPR) + tid / S::LPR, c = tid % S::LPR;
-        put(kl + k_at<HD>(row, MX ? 2 * c : c), t.k[j], MX ? t.ks[j] : 0u);
-        put(vl + v_at<HD>(row, MX ? 2 * c : c), t.v[j], MX ? t.vs[j] : 0u);
+        put(kl + k_at<HD>(row, MX ? 2 * c : c), t.k[j], MX ? t.ks[j] : 0u, c / 2);
+        put(vl + v_at<HD>(row, MX ? 2 * c : c), t.v[j], MX ? t.vs[j] : 0u, c / 2);
     }
 }
 
@@ -759,7 +770,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
-    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, p.per_split);
     const int t_begin = split * per, t_end = min(tiles, t_begin + per);
     // what the rows of this wave see at least and at most (its rows may lie beyond the group's end)
     const int w0 = r0 + 16 * MT * wave, w1 = min(r_end - 1, w0 + 16 * MT - 1);
@@ -927,14 +938,29 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     }
 }
 
-// ---- hundreds of query rows per group: bound by the matrix pipe, with the vector pipe (softmax) and the LDS close behind.
-// Workgroup = (group, block of 256 rows, key range), two halves of four waves; wave = 32 rows.  A tile costs a wave a MATRIX phase (the product
-// with the previous tile's values, then the scores of this one: 68 MFMAs) and a VECTOR phase (softmax, staging) of about the same length.
-// The halves run one phase apart, so that on every SIMD one wave is in its matrix phase while the other is in its vector phase; a barrier
-// ends each phase.  Phase 2 t: half 0 multiplies (values of t - 1, keys of t); phase 2 t + 1: half 1 does.  Keys of tile t are read in
-// phases 2 t and 2 t + 1, values in 2 t + 2 and 2 t + 3; each half stages its 32 rows of a tile in its vector phases: half h, after the
-// scores of tile t, keys of t + 1 + h and values of t + h - two LDS buffers each, always written after their last reader's barrier.
-// The row sums come from the matrix pipe as well (a product of P with ones: 4 of the 68 MFMAs instead of 32 additions).
+// ---- hundreds of query rows per group: bound by what two waves per SIMD can issue (matrix products, exponentials, and every other
+// instruction of the softmax and of widening a tile).
+// Workgroup = (group, block of 256 rows, key range), two halves of four waves; wave = 32 rows on 32 x 32 x 16 products (half the instructions
+// of 16 x 16 ones, and a lane has one query: S^T = K Q^T puts keys 8 (r >> 2) + 4 h + (r & 3) of query lane & 31 into register r, h = lane >> 5,
+// which eight at a time are the P^T operand of O^T = V^T P^T).  A tile costs a wave a MATRIX phase (the product with the previous tile's
+// values, then the scores of this one) and a VECTOR phase (softmax, staging) of about the same length.  The halves run one phase apart, so
+// that on every SIMD one wave is in its matrix phase while the other is in its vector phase; a barrier ends each phase.  Phase 2 t: half 0
+// multiplies (values of t - 1, keys of t); phase 2 t + 1: half 1 does.  Keys of tile t are read in phases 2 t and 2 t + 1, values in 2 t + 2
+// and 2 t + 3; each half stages its 32 rows of a tile in its vector phases: half h, after the scores of tile t, keys of t + 1 + h and
+// values of t + h - two LDS buffers each, always written after their last reader's barrier.
+// Tiles that every row of the block sees whole take a loop without masks and case distinctions (a lone wave issues an instruction every
+// five to six cycles, scalar ones too: it is their number that counts).
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+SEEDMI_DEVINL f32x16 mfma_32x32x16(bf16x8 a, bf16x8 b, f32x16 c) {
+#ifdef SEEDMI_F16
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(hw_f16x8, a), __builtin_bit_cast(hw_f16x8, b), c, 0, 0, 0);
+#else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+#endif
+}
+template <int HD>
+SEEDMI_DEVINL constexpr int w_at(int row, int c) { return row * (2 * HD + 64) + 16 * c; }      // value rows here: 64 bytes of 4 rows at a time
+
 template <int HD, bool MX>
 struct HalfStage {                                       // a thread's part of 32 rows of K and V
     static constexpr int RB = MX ? HD : 2 * HD;
@@ -943,14 +969,16 @@ struct HalfStage {                                       // a thread's part of 3
     uint4 k[L], v[L];
     uint32_t ks[L], vs[L];
 };
+struct WholeTile { static constexpr bool value = true; };                // every row of the block sees all of the tile
+struct AnyTile { static constexpr bool value = false; };
 
 template <int HD, bool MX>
 __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs a) {
-    constexpr int MT = 2, NT = HD / 16, KS = HD / 32;
-    constexpr int KB = k_at<HD>(KT2, 0), VB = v_at<HD>(KT2, 0);          // bytes of the images
+    constexpr int NT = HD / 32, KS = HD / 16;
+    constexpr int KB = k_at<HD>(KT2, 0), VB = w_at<HD>(KT2, 0);          // bytes of the images
     __shared__ __attribute__((aligned(16))) char sm[2 * KB + 4 * VB];    // K0 K1, V0 V1, raw V0 V1
     __shared__ int s_bad;                                // a tile that some row does not see whole held a value that is not finite
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g4 = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2, ht = tid & 255;
     unsigned block;
     const AttnPass p = pass_of(a, block);
@@ -971,33 +999,33 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? len - a.T + r0 / a.GH + 1 : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
-    const int per = max((tiles + p.splits - 1) / p.splits, MIN_TILES);
+    const int per = max((tiles + p.splits - 1) / p.splits, p.per_split);
     const int t0 = split * per, n = max(0, min(tiles, t0 + per) - t0);   // first tile, number of tiles
     const int w0 = r0 + 32 * wave, w1 = min(r_end - 1, w0 + 31);
-    const int wave_max = w0 >= r_end ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
-    const int wave_min = w0 >= r_end ? 0 : causal ? len - a.T + w0 / a.GH + 1 : len;
+    const bool active = w0 < r_end;                      // the wave has rows
+    const int wave_max = !active ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
+    const int wave_min = !active ? 0 : causal ? len - a.T + w0 / a.GH + 1 : len;
 
-    bf16x8 qf[MT][KS];
-    int seen[MT];
-    float m[MT];
-    f32x4 o[MT][NT], l[MT];
-#pragma unroll
-    for (int u = 0; u < MT; ++u) {
-        const int r = w0 + 16 * u + li;
-        const bool on = r < r_end;
-        seen[u] = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
-        const bf16_t* qp = a.q + (size_t)(base + (on ? r / a.GH : 0)) * a.ldq + (kvh * a.GH + (on ? r % a.GH : 0)) * HD;
+    const int r = w0 + lq;                               // this lane's query row
+    const bool on = r < r_end;
+    const int token = base + (on ? r / a.GH : 0), head = kvh * a.GH + (on ? r % a.GH : 0);
+    const int seen = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
+    bf16x8 qf[1][KS];
+    {
+        const bf16_t* qp = a.q + (size_t)token * a.ldq + head * HD + 8 * h;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (on) v = *(const uint4*)(qp + 32 * ks + 8 * g4);
-            qf[u][ks] = __builtin_bit_cast(bf16x8, v);
+            if (on) v = *(const uint4*)(qp + 16 * ks);
+            qf[0][ks] = __builtin_bit_cast(bf16x8, v);
         }
-        m[u] = -INFINITY;
-        l[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NT; ++i) o[u][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[i][d] = 0.f;
     const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = HalfStage<HD, MX>;
     const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
@@ -1005,16 +1033,17 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
 
     arrived(qf);
-    constexpr int KP = k_at<HD>(1, 0), VP = v_at<HD>(1, 0);              // row pitches of the images
+    constexpr int KP = k_at<HD>(1, 0), VP = w_at<HD>(1, 0);              // row pitches of the images
     S st;
+    // tiles from n on: behind the last row, nothing is fetched
     auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const __amdgpu_buffer_rsrc_t& b, const __amdgpu_buffer_rsrc_t& sb, int t) {
         if (!stages) return;
         const int key0 = (t < n ? t0 + t : tiles) * KT2;
 #pragma unroll
         for (int j = 0; j < S::L; ++j) {
-            const int r = srow + j * (256 / S::LPR);
-            w[j] = load16(b, r * S::RB + 16 * schunk, key0 * S::RB);
-            if (MX) sc[j] = __builtin_amdgcn_raw_buffer_load_b8(sb, r * (HD / 32) + schunk / 2, key0 * (HD / 32), 0);
+            const int row = srow + j * (256 / S::LPR);
+            w[j] = load16(b, row * S::RB + 16 * schunk, key0 * S::RB);
+            if (MX) sc[j] = load_scale<HD>(sb, row, schunk / 2, key0 * (HD / 32));
         }
     };
     // raw: where a value tile that some row does not see whole leaves its rows as they are; the image then holds zeros in place of what is not
@@ -1034,7 +1063,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         for (int j = 0; j < S::L; ++j) {
             const int at = (srow + j * (256 / S::LPR)) * pitch + (MX ? 32 : 16) * schunk;
             if (MX) {
-                const float s = mx_scale_f(sc[j]);
+                const float s = scale_of<HD>(sc[j], schunk / 2);
                 put(at, make_uint4(mx_unpack2<false>(w[j].x, s), mx_unpack2<true>(w[j].x, s), mx_unpack2<false>(w[j].y, s), mx_unpack2<true>(w[j].y, s)));
                 put(at + 16, make_uint4(mx_unpack2<false>(w[j].z, s), mx_unpack2<true>(w[j].z, s), mx_unpack2<false>(w[j].w, s), mx_unpack2<true>(w[j].w, s)));
             } else {
@@ -1045,8 +1074,8 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     };
     auto kbuf = [&](int t) { return sm + (t & 1) * KB; };
     auto vbuf = [&](int t) { return sm + 2 * KB + (t & 1) * VB; };
-    auto mixed_tile = [&](int t) { return (t0 + t + 1) * KT2 > n_min; }; // some row of the block does not see all of it
-    auto vraw = [&](int t) { return mixed_tile(t) ? sm + 2 * KB + (2 + (t & 1)) * VB : nullptr; };
+    auto partial_tile = [&](int t) { return (t0 + t + 1) * KT2 > n_min; };               // some row of the block does not see all of it
+    auto vraw = [&](int t) { return partial_tile(t) ? sm + 2 * KB + (2 + (t & 1)) * VB : nullptr; };
 
     if (tid == 0) s_bad = 0;
     __syncthreads();
@@ -1056,7 +1085,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         if (half) {                                      // half 1 is one vector phase ahead in its staging
             load_rows(st.k, st.ks, rows.k, rows.ks, 1);
             load_rows(st.v, st.vs, rows.v, rows.vs, 0);
-            if (n > 1) store_rows(st.k, st.ks, kbuf(1), KP, nullptr);
+            store_rows(st.k, st.ks, kbuf(1), KP, nullptr);
             store_rows(st.v, st.vs, vbuf(0), VP, vraw(0));
         }
         load_rows(st.k, st.ks, rows.k, rows.ks, 1 + half);
@@ -1064,132 +1093,139 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     }
     __syncthreads();
 
-    bf16x8 pf[MT][2];
-    auto values = [&](int t) {                           // o += P V, l += P 1 for the tile whose probabilities are in pf
-        const char* vl = vbuf(t);
-        const bf16x8 ones = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(1.f, 1.f), pack2bf(1.f, 1.f), pack2bf(1.f, 1.f), pack2bf(1.f, 1.f)));
+    bf16x8 pf[4];                                        // P^T of a tile, 16 keys each
+    const int vlane = w_at<HD>(4 * h + ((lane & 15) >> 2), 0) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    auto values = [&](int t) {                           // o += P V for the tile whose probabilities are in pf
+        const char* vl = vbuf(t) + vlane;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const bf16x8 vf = v_frag<HD>(vl + v_at<HD>(32 * kk, 0), i, lane);
-#pragma unroll
-                for (int u = 0; u < MT; ++u) o[u][i] = seedmi_mfma_16x16x32(vf, pf[u][kk], o[u][i]);
+                // channels 32 i + (lane & 31), keys 16 ks + 4 h + (j & 3) + 8 (j >> 2)
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vl + w_at<HD>(16 * ks, 4 * i)));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vl + w_at<HD>(16 * ks + 8, 4 * i)));
+                const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
+                o[i] = mfma_32x32x16(__builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pf[ks], o[i]);
             }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-            for (int u = 0; u < MT; ++u) l[u] = seedmi_mfma_16x16x32(ones, pf[u][kk], l[u]);
-        if (__builtin_expect(mixed_tile(t) && __builtin_amdgcn_readfirstlane(s_bad), 0)) {
-            const int g = fresh_lane() >> 4;
-            const char* rl = sm + 2 * KB + (2 + (t & 1)) * VB;
-#pragma unroll 1
-            for (int j = 0; j < KT2; ++j) {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const uint2 w = *(const uint2*)(rl + v_at<HD>(j, 2 * i) + 8 * g);
-                    const uint32_t h[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int u = 0; u < MT; ++u)
-                            if (bad16(h[r]) && (t0 + t) * KT2 + j < seen[u]) o[u][i][r] += bf2f((bf16_t)h[r]);
-                }
-            }
-        }
     };
-
-    if (half) __syncthreads();                           // phase 0 belongs to half 0
+    auto values_not_finite = [&](int t) {                // see kv_attention_few_kernel
+        if (__builtin_amdgcn_readfirstlane(s_bad) == 0) return;
+        const int hh = fresh_lane() >> 5;
+        const char* rl = sm + 2 * KB + (2 + (t & 1)) * VB;
 #pragma unroll 1
-    for (int t = 0; t < n; ++t) {
-        const int key0 = (t0 + t) * KT2;
-        // ---- matrix phase
-        __builtin_amdgcn_s_setprio(1);
-        f32x4 s[MT][4];
-        const bool live = key0 < wave_max;               // (wave-uniform; tiles are in order: once dead, dead to the end)
-        if (t > 0 && key0 - KT2 < wave_max) values(t - 1);
-        if (live) {
-            const char* kl = kbuf(t);
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                bf16x8 kf[KS];
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const bf16x8*)(kl + k_at<HD>(16 * kt + li, 4 * ks + g4));
-#pragma unroll
-                for (int u = 0; u < MT; ++u) {
-                    s[u][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) s[u][kt] = seedmi_mfma_16x16x32(kf[ks], qf[u][ks], s[u][kt]);
-                }
-            }
-        }
-        __builtin_amdgcn_s_setprio(0);
-        __syncthreads();
-        // ---- vector phase
-        if (t + 1 + half < n) store_rows(st.k, st.ks, kbuf(t + 1 + half), KP, nullptr);
-        if (t + half < n) store_rows(st.v, st.vs, vbuf(t + half), VP, vraw(t + half));
-        load_rows(st.k, st.ks, rows.k, rows.ks, t + 2 + half);
-        load_rows(st.v, st.vs, rows.v, rows.vs, t + 1 + half);
-        if (live) {
-#pragma unroll
-            for (int u = 0; u < MT; ++u) {
-                if (key0 + KT2 > wave_min) {
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (key0 + 16 * kt + 4 * g4 + r >= seen[u]) s[u][kt][r] = -INFINITY;
-                }
-                float tm = -INFINITY;
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt) tm = fmaxf(tm, fmaxf(fmaxf(s[u][kt][0], s[u][kt][1]), fmaxf(s[u][kt][2], s[u][kt][3])));
-                tm = rows_max(tm) * a.c2;
-                const float mn = fmaxf(m[u], tm);
-                if (__any(mn > m[u])) {
-                    const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) l[u][r] *= f;
-#pragma unroll
-                    for (int i = 0; i < NT; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[u][i][r] *= f;
-                    m[u] = mn;
-                }
-                const float ref = mn == -INFINITY ? 0.f : mn;
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    float e[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
-                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
-                }
-            }
-        }
-        __syncthreads();
-    }
-    if (n > 0 && (t0 + n - 1) * KT2 < wave_max) values(n - 1);
-    if (!half) __syncthreads();                          // (half 1's last vector phase)
-
-#pragma unroll
-    for (int u = 0; u < MT; ++u) {
-        const float L = l[u][0];
-        const int r = w0 + 16 * u + li;
-        if (r >= r_end) continue;
-        const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
-        if (a.parts == 1) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
+        for (int j = 0; j < KT2; ++j) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
-                *(uint2*)(op + 16 * i) = make_uint2(pack2bf(o[u][i][0] * inv, o[u][i][1] * inv), pack2bf(o[u][i][2] * inv, o[u][i][3] * inv));
-        } else {
-            const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
-            if (L != 0.f) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i) *(f32x4*)(a.o_part + at * HD + 16 * i + 4 * g4) = o[u][i];
-            }
-            if (g4 == 0) a.ml_part[at] = make_float2(fmaxf(m[u], LOWEST), L);
+                for (int e = 0; e < 4; ++e) {
+                    const uint2 w = *(const uint2*)(rl + w_at<HD>(j, 4 * i + e) + 8 * hh);
+                    const uint32_t x[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        if (bad16(x[d]) && (t0 + t) * KT2 + j < seen) o[i][4 * e + d] += bf2f((bf16_t)x[d]);
+                }
         }
+    };
+    const int klane = k_at<HD>(lq, h);
+    f32x16 s[2];
+    auto scores = [&](int t) {
+        const char* kl = kbuf(t) + klane;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d) s[kt][d] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[kt] = mfma_32x32x16(*(const bf16x8*)(kl + k_at<HD>(32 * kt, 2 * ks)), qf[0][ks], s[kt]);
+        }
+    };
+    auto softmax = [&](int key0, bool masked) {
+        if (masked) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int d = 0; d < 16; ++d)
+                    if (key0 + 32 * kt + 8 * (d >> 2) + 4 * h + (d & 3) >= seen) s[kt][d] = -INFINITY;
+        }
+        float tm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int d = 1; d < 16; ++d) tm = fmaxf(tm, fmaxf(s[0][d], s[1][d]));
+        auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
+        tm = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c2;
+        const float mn = fmaxf(m, tm);
+        if (__any(mn > m)) {
+            const float f = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int d = 0; d < 16; ++d) o[i][d] *= f;
+            m = mn;
+        }
+        const float ref = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], a.c2, -ref));
+                l += e[j];
+            }
+            pf[ks] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
+        }
+    };
+    auto step = [&](auto whole, int t) {                 // matrix phase and vector phase of tile t
+        constexpr bool W = decltype(whole)::value;       // (tiles before a whole one are whole)
+        const int key0 = (t0 + t) * KT2;
+        const bool live = W ? active : key0 < wave_max;  // (wave-uniform; tiles are in order: once dead, dead to the end)
+        __builtin_amdgcn_s_setprio(1);
+        if (t > 0 && (W ? active : key0 - KT2 < wave_max)) {
+            values(t - 1);
+            if (!W && partial_tile(t - 1)) values_not_finite(t - 1);
+        }
+        if (live) scores(t);
+        __builtin_amdgcn_s_setprio(0);
+        __syncthreads();
+        store_rows(st.k, st.ks, kbuf(t + 1 + half), KP, nullptr);
+        store_rows(st.v, st.vs, vbuf(t + half), VP, W ? nullptr : vraw(t + half));
+        load_rows(st.k, st.ks, rows.k, rows.ks, t + 2 + half);
+        load_rows(st.v, st.vs, rows.v, rows.vs, t + 1 + half);
+        if (live) softmax(key0, W ? false : key0 + KT2 > wave_min);
+        __syncthreads();
+    };
+    // the whole tiles, less the last of them: a vector phase stages values of up to one tile later
+    const int whole = max(0, min(n, n_min / KT2 - t0) - 1);
+    if (half) __syncthreads();                           // phase 0 belongs to half 0
+#pragma unroll 1
+    for (int t = 0; t < whole; ++t) step(WholeTile(), t);
+#pragma unroll 1
+    for (int t = whole; t < n; ++t) step(AnyTile(), t);
+    if (n > 0 && (t0 + n - 1) * KT2 < wave_max) {
+        values(n - 1);
+        if (partial_tile(n - 1)) values_not_finite(n - 1);
+    }
+    if (!half) __syncthreads();                          // (half 1's last vector phase)
+
+    auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    const float L = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    if (!on) return;
+    if (a.parts == 1) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * h;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *(uint2*)(op + 32 * i + 8 * e) = make_uint2(pack2bf(o[i][4 * e] * inv, o[i][4 * e + 1] * inv), pack2bf(o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv));
+    } else {
+        const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
+        if (L != 0.f) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    *(f32x4*)(a.o_part + at * HD + 32 * i + 8 * e + 4 * h) = (f32x4){o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
+        }
+        if (h == 0) a.ml_part[at] = make_float2(fmaxf(m, LOWEST), L);
     }
 }
 
@@ -1337,7 +1373,7 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
 }
 
 // How a call is cut: a pass over the slots' own rows and, with a prefix, one over the prefix; row blocks and key ranges of each.
-struct KvPass { int groups, group_rows, block_rows, row_blocks, splits; unsigned blocks; };
+struct KvPass { int groups, group_rows, block_rows, row_blocks, splits, per_split; unsigned blocks; };
 struct KvPlan {
     KvPass own, pre;
     int parts, units, unit_rows;                         // units > 0: joined in place, by the last workgroup of each unit
@@ -1360,6 +1396,8 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);
+    p.per_split = (int)((tiles + p.splits - 1) / p.splits);
+    if (p.per_split < MIN_TILES) p.per_split = MIN_TILES;
     p.blocks = ((unsigned)p.groups * p.splits + 7) / 8 * 8 * p.row_blocks;
     return p;
 }
@@ -1431,7 +1469,7 @@ template <int HD, bool MX>
 static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, const KvPlan& pl, int prefix_len, int kv_len, const int* kv_lens,
                              hipStream_t s) {
     auto set = [](AttnPass& x, const KvView& v, const KvPass& p, int shared, int part0, int len, const int* lens) {
-        x = {v, lens, len, shared, p.groups, p.group_rows, p.row_blocks, p.splits, part0, p.blocks};
+        x = {v, lens, len, shared, p.groups, p.group_rows, p.row_blocks, p.splits, part0, p.per_split, p.blocks};
     };
     if (!prefix_len) {
         set(a.pass[0], own, pl.own, 0, 0, kv_len, kv_lens);
