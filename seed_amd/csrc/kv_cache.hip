@@ -223,12 +223,15 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr int KT = 32;                                   // keys of a tile
 constexpr int MIN_TILES = 4;                             // of a split: one tile per wave
 
+// maximum of three that a NaN goes through (v_maximum3_f32; fmaxf would quieten each of its operands first: three instructions for one)
+SEEDMI_DEVINL float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
+SEEDMI_DEVINL float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // maximum / sum over the four 16-lane rows of a wave (the lanes of one query): VALU row swaps, no LDS
 SEEDMI_DEVINL float rows_max(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    x = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 SEEDMI_DEVINL float rows_sum(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -578,8 +581,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
                     for (int r = 0; r < 4; ++r)
                         if (key0 + 16 * kt + 4 * g4 + r >= seen[u]) s[u][kt][r] = -INFINITY;
             }
-            float tm = fmaxf(fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][0][2], s[u][0][3])),
-                             fmaxf(fmaxf(s[u][1][0], s[u][1][1]), fmaxf(s[u][1][2], s[u][1][3])));
+            float tm = max3(max3(s[u][0][0], s[u][0][1], s[u][0][2]), max3(s[u][0][3], s[u][1][0], s[u][1][1]), max2(s[u][1][2], s[u][1][3]));
             tm = rows_max(tm) * a.c2;
             const float mn = fmaxf(m[u], tm);
             if (__any(mn > m[u])) {                      // a new maximum: what is summed so far is scaled down
@@ -855,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
                 }
                 float tm = -INFINITY;
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) tm = fmaxf(tm, fmaxf(fmaxf(s[u][kt][0], s[u][kt][1]), fmaxf(s[u][kt][2], s[u][kt][3])));
+                for (int kt = 0; kt < 4; ++kt) tm = max3(max3(tm, s[u][kt][0], s[u][kt][1]), s[u][kt][2], s[u][kt][3]);
                 tm = rows_max(tm) * a.c2;
                 const float mn = fmaxf(m[u], tm);
                 if (__any(mn > m[u])) {
@@ -958,6 +960,14 @@ SEEDMI_DEVINL f32x16 mfma_32x32x16(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 #endif
 }
+// acc + lo + hi of a word of two 16-bit elements: a dot product with ones
+SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
+#ifdef SEEDMI_F16
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(hw_f16x2, w), __builtin_bit_cast(hw_f16x2, 0x3c003c00u), acc, false);
+#else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, w), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), acc, false);
+#endif
+}
 template <int HD>
 SEEDMI_DEVINL constexpr int w_at(int row, int c) { return row * (2 * HD + 64) + 16 * c; }      // value rows here: 64 bytes of 4 rows at a time
 
@@ -1034,9 +1044,9 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 
     arrived(qf);
     constexpr int KP = k_at<HD>(1, 0), VP = w_at<HD>(1, 0);              // row pitches of the images
-    S st;
+    S st;                                                // (a second set, requested two tiles ahead: no faster)
     // tiles from n on: behind the last row, nothing is fetched
-    auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const __amdgpu_buffer_rsrc_t& b, const __amdgpu_buffer_rsrc_t& sb, int t) {
+    auto load_rows = [&](uint4 (&w)[S::L], uint32_t (&sc)[S::L], const __amdgpu_buffer_rsrc_t& b, const __amdgpu_buffer_rsrc_t& sb, int t) __attribute__((always_inline)) {
         if (!stages) return;
         const int key0 = (t < n ? t0 + t : tiles) * KT2;
 #pragma unroll
@@ -1048,7 +1058,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     };
     // raw: where a value tile that some row does not see whole leaves its rows as they are; the image then holds zeros in place of what is not
     // finite (0 * inf must not reach a row that does not see the key; the rows that do take it from the raw rows)
-    auto store_rows = [&](const uint4 (&w)[S::L], const uint32_t (&sc)[S::L], char* dst, int pitch, char* raw) {
+    auto store_rows = [&](const uint4 (&w)[S::L], const uint32_t (&sc)[S::L], char* dst, int pitch, char* raw) __attribute__((always_inline)) {
         if (!stages) return;
         bool bad = false;
         auto put = [&](int at, uint4 x) {
@@ -1095,7 +1105,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 
     bf16x8 pf[4];                                        // P^T of a tile, 16 keys each
     const int vlane = w_at<HD>(4 * h + ((lane & 15) >> 2), 0) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-    auto values = [&](int t) {                           // o += P V for the tile whose probabilities are in pf
+    auto values = [&](int t) __attribute__((always_inline)) {                           // o += P V for the tile whose probabilities are in pf
         const char* vl = vbuf(t) + vlane;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
@@ -1108,7 +1118,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 o[i] = mfma_32x32x16(__builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y)), pf[ks], o[i]);
             }
     };
-    auto values_not_finite = [&](int t) {                // see kv_attention_few_kernel
+    auto values_not_finite = [&](int t) __attribute__((always_inline)) {                // see kv_attention_few_kernel
         if (__builtin_amdgcn_readfirstlane(s_bad) == 0) return;
         const int hh = fresh_lane() >> 5;
         const char* rl = sm + 2 * KB + (2 + (t & 1)) * VB;
@@ -1128,17 +1138,16 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     };
     const int klane = k_at<HD>(lq, h);
     f32x16 s[2];
-    auto scores = [&](int t) {
+    auto scores = [&](int t) __attribute__((always_inline)) {
         const char* kl = kbuf(t) + klane;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int d = 0; d < 16; ++d) s[0][d] = s[1][d] = 0.f;
 #pragma unroll
-            for (int d = 0; d < 16; ++d) s[kt][d] = 0.f;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[kt] = mfma_32x32x16(*(const bf16x8*)(kl + k_at<HD>(32 * kt, 2 * ks)), qf[0][ks], s[kt]);
-        }
+            for (int kt = 0; kt < 2; ++kt) s[kt] = mfma_32x32x16(*(const bf16x8*)(kl + k_at<HD>(32 * kt, 2 * ks)), qf[0][ks], s[kt]);
     };
-    auto softmax = [&](int key0, bool masked) {
+    auto softmax = [&](int key0, bool masked) __attribute__((always_inline)) {
         if (masked) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -1146,12 +1155,12 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 for (int d = 0; d < 16; ++d)
                     if (key0 + 32 * kt + 8 * (d >> 2) + 4 * h + (d & 3) >= seen) s[kt][d] = -INFINITY;
         }
-        float tm = fmaxf(s[0][0], s[1][0]);
+        float tm = max2(s[0][0], s[1][0]);
 #pragma unroll
-        for (int d = 1; d < 16; ++d) tm = fmaxf(tm, fmaxf(s[0][d], s[1][d]));
+        for (int d = 1; d < 16; ++d) tm = max3(tm, s[0][d], s[1][d]);
         auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
-        tm = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c2;
-        const float mn = fmaxf(m, tm);
+        tm = max2(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c2;
+        const float mn = fmaxf(m, tm);                   // (a NaN among the scores is in the sums, whatever the maximum)
         if (__any(mn > m)) {
             const float f = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
             l *= f;
@@ -1166,23 +1175,42 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         for (int ks = 0; ks < 4; ++ks) {
             float e[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], a.c2, -ref));
-                l += e[j];
-            }
-            pf[ks] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
+            for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], a.c2, -ref));
+            const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
+            l = add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, l))));           // (the rounded ones, as the product takes them)
+            pf[ks] = __builtin_bit_cast(bf16x8, w);
         }
     };
-    auto step = [&](auto whole, int t) {                 // matrix phase and vector phase of tile t
+    auto step = [&](auto whole, int t) __attribute__((always_inline)) {                 // matrix phase and vector phase of tile t
         constexpr bool W = decltype(whole)::value;       // (tiles before a whole one are whole)
         const int key0 = (t0 + t) * KT2;
         const bool live = W ? active : key0 < wave_max;  // (wave-uniform; tiles are in order: once dead, dead to the end)
         __builtin_amdgcn_s_setprio(1);
-        if (t > 0 && (W ? active : key0 - KT2 < wave_max)) {
-            values(t - 1);
-            if (!W && partial_tile(t - 1)) values_not_finite(t - 1);
+        if (W) {
+            if (live) {
+                values(t - 1);
+                scores(t);
+                // fragments are read four products ahead of their use (left alone, the compiler reads two, waits, and multiplies twice)
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+                for (int i = 0; i < 4 * NT - 4; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * KS; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            }
+        } else {
+            if (t > 0 && key0 - KT2 < wave_max) {
+                values(t - 1);
+                if (partial_tile(t - 1)) values_not_finite(t - 1);
+            }
+            if (live) scores(t);
         }
-        if (live) scores(t);
         __builtin_amdgcn_s_setprio(0);
         __syncthreads();
         store_rows(st.k, st.ks, kbuf(t + 1 + half), KP, nullptr);
@@ -1193,12 +1221,14 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         __syncthreads();
     };
     // the whole tiles, less the last of them: a vector phase stages values of up to one tile later
-    const int whole = max(0, min(n, n_min / KT2 - t0) - 1);
+    const int whole = min(n, n_min / KT2 - t0) - 1;
     if (half) __syncthreads();                           // phase 0 belongs to half 0
 #pragma unroll 1
-    for (int t = 0; t < whole; ++t) step(WholeTile(), t);
+    for (int t = 0; t < n;) {
+        step(AnyTile(), t++);                            // the first (no values before it) ...
 #pragma unroll 1
-    for (int t = whole; t < n; ++t) step(AnyTile(), t);
+        while (t < whole) step(WholeTile(), t++);
+    }                                                    // ... and those at the end
     if (n > 0 && (t0 + n - 1) * KT2 < wave_max) {
         values(n - 1);
         if (partial_tile(n - 1)) values_not_finite(n - 1);

@@ -345,6 +345,25 @@ def test_peaked_and_flat_scores(gain):
             _check(out, q, per_slot, None, H, H, T, 0.25, True, f"{fmt} T {T}")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T", [1, 20, 100, 300])
+def test_many_small_probabilities_count(dtype, T):
+    """One key ahead of 1500 others whose probabilities, 2^-15.5 and less each, are fp16's subnormal numbers and together a part of the sum."""
+    H, D, n = 1, 128, 1800
+    cache = _poisoned(1, H, n, D, "16", dtype)
+    k = torch.zeros(H, n, D)
+    k[:, :, 0] = -1.0 - torch.arange(n) % 7 / 64.0
+    k[:, 5, 0] = 0.0
+    v = torch.ones(H, n, D)
+    v[:, 5] = 0.0
+    cache.k[0], cache.v[0] = k.to(dtype).cuda(), v.to(dtype).cuda()
+    q = torch.zeros(T, H * D)
+    q[:, 0] = 10.75                                                                # exp(-10.75) = 2^-15.51
+    q = q.to(dtype).cuda()
+    out = KVAttention(cache, heads=H, tokens=T, scale=1.0)(q, n)
+    _check(out, q, [(k.to(dtype).double(), v.to(dtype).double())], None, H, H, T, 1.0, True)
+
+
 def test_lengths_beyond_the_cache_are_clamped():
     H, D = 2, 128
     cache = _poisoned(2, H, 70, D, "mx8", BF)
