@@ -490,8 +490,8 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     const unsigned item = blk * 8 + in % 8;
     const int rb = in / 8;
     if (item >= items) return;
-    const int split = item / p.groups, group = item % p.groups;
-    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int G = p.c.G, split = item / p.groups, group = (int)((item % p.groups + (unsigned)split * G) % p.groups);    // (see plan_pass)
+    const int slot = group / G, kvh = group % G;
     const int base = p.shared ? 0 : slot * a.T;          // first token row of the group
     const int r0 = rb * 16 * MT, r_end = min(p.group_rows, r0 + 16 * MT);
 
@@ -761,8 +761,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     const unsigned item = blk * 8 + in % 8;
     const int rb = p.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
     if (item >= items) return;
-    const int split = item / p.groups, group = item % p.groups;
-    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int G = p.c.G, split = item / p.groups, group = (int)((item % p.groups + (unsigned)split * G) % p.groups);    // (see plan_pass)
+    const int slot = group / G, kvh = group % G;
     const int base = p.shared ? 0 : slot * a.T;
     const int r0 = rb * 64 * MT, r_end = min(p.group_rows, r0 + 64 * MT);
 
@@ -997,8 +997,8 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const unsigned item = blk * 8 + in % 8;
     const int rb = p.row_blocks - 1 - (int)(in / 8);     // (causal: the longest ranges first)
     if (item >= items) return;
-    const int split = item / p.groups, group = item % p.groups;
-    const int G = p.c.G, slot = group / G, kvh = group % G;
+    const int G = p.c.G, split = item / p.groups, group = (int)((item % p.groups + (unsigned)split * G) % p.groups);    // (see plan_pass)
+    const int slot = group / G, kvh = group % G;
     const int base = p.shared ? 0 : slot * a.T;
     const int r0 = rb * 256, r_end = min(p.group_rows, r0 + 256);
 
@@ -1422,7 +1422,9 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     const int kt = p.block_rows <= 32 ? KT : KT2;
     const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
-    const long long target = 256;                                         // one workgroup per CU: more ranges cost more in parts than they balance
+    // One workgroup per CU, two of the 64- and 128-row ones (they share a CU).  A range has a fixed number of tiles (of the longest slot
+    // expected), so short slots have fewer; the slots take turns from range to range, so that the CUs get as many of them each.
+    const long long target = p.block_rows == 64 || p.block_rows == 128 ? 512 : 256;
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
     p.splits = (int)(s < 1 ? 1 : s);
