@@ -311,9 +311,10 @@ int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv, int ldqkv,
 int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int B, int n, int start, const void* starts_i32, void* stream);
 /* Attention of T query rows per slot over the slot's cache rows, H query heads on kv_heads key heads (head h reads key head
  * h / (H / kv_heads)): out = softmax(scale * q k^T) v.  q and out are [B*T, H * head_dim] (row strides ldq, ldo).  Slot b holds
- * n_b = kv_lens_i32[b] rows (device int32 [B]; kv_len when that is NULL), the T queries are its last rows: with causal != 0 query t sees
- * rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all visible) rows 0 .. n_b - 1.  n_b is clamped to
- * [0, cache->rows]; scale is finite and above 0.  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
+ * n_b = kv_len rows, or kv_lens_i32[b] + kv_len where kv_lens_i32 (device int32 [B]) is given - kv_len = T with the lengths that
+ * seedmi_kv_append took, 0 with lengths that count the new rows already - and none where kv_lens_i32[b] is negative (idle).  The T queries
+ * are the slot's last rows: with causal != 0 query t sees rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all
+ * visible) rows 0 .. n_b - 1.  n_b is clamped to [0, cache->rows]; scale is finite and above 0.  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
  * head_dim), in front of its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros.
  * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the
  * probabilities (unnormalised, 0 .. 1) are rounded to the 16-bit element for the product with the values.
@@ -514,6 +515,17 @@ int seedmi_llama_forward_io(const seedmi_llama_weights_t* w, const void* ids_i64
  * position of every slot).  Rows are independent: an idle slot (length 0, any token) costs its share of the weight stream only. */
 int seedmi_llama_decode_slots(const seedmi_llama_weights_t* w, const void* tok_i64, const void* lens_i32, int batch, void* logits,
                               int ldl, void* workspace, size_t workspace_bytes, void* stream);
+/* LlamaForCausalLM.forward over cache handles instead of the layers' static caches: kv is a host array [layers] of caches (kv_heads = heads,
+ * head_dim as the model's, any format) whose slot b holds past_lens_i32[b] rows (device int32 [batch]; negative: an idle slot, its logits
+ * mean nothing); T new positions per slot are appended and attended to, behind rows 0 .. prefix_len - 1 of slot 0 of prefix[layer] when
+ * prefix_len > 0 (a prompt that all slots share; prefix is a host array [layers] or NULL).  Positions are prefix_len + past + t.  past_max:
+ * the longest past expected (host), for the position check and the split of the keys.  Everything else is seedmi_llama_forward: the same
+ * GEMMs on the same workspace, T = 1 the decode path.  No launch argument depends on the lengths: a captured step replays as they grow.
+ * attn_workspace: seedmi_kv_attention_workspace_bytes(&kv[0], batch, T, heads, past_max + T, prefix_len) bytes, initialised once. */
+int seedmi_llama_forward_kv(const seedmi_llama_weights_t* w, const seedmi_kv_cache_t* kv, const seedmi_kv_cache_t* prefix, int prefix_len,
+                            const void* ids_i64, int batch, int T, const void* past_lens_i32, int past_max, int last_only, void* logits,
+                            int ldl, void* attn_workspace, size_t attn_workspace_bytes, void* workspace, size_t workspace_bytes,
+                            void* stream);
 /* seedmi_gemm_skinny_ws_status for the split-K area inside a decode workspace (the one passed to the T = 1 forward / decode_slots calls
  * of this batch): SEEDMI_OK when every decode step since the last check completed its cut tiles, SEEDMI_E_HIP otherwise (the logits of
  * those steps are then invalid).  SYNCHRONISES `stream`; a decode loop calls it once at its end (seed_amd/llama_engine.py does). */

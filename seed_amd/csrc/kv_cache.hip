@@ -219,6 +219,16 @@ SEEDMI_DEVINL AttnPass pass_of(const AttnArgs& a, unsigned& block) {
     return p;
 }
 
+// rows of a pass's slot that count: kv_len, on top of what the slot's own length says where there is one (negative: an idle slot), within the cache
+SEEDMI_DEVINL int rows_held(const AttnPass& p, int slot) {
+    int n = p.kv_len;
+    if (p.kv_lens && !p.shared) {
+        const int own = p.kv_lens[slot];
+        n = own < 0 ? 0 : min(own, p.c.rows) + n;
+    }
+    return __builtin_amdgcn_readfirstlane(max(0, min(n, p.c.rows)));
+}
+
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr int KT = 32;                                   // keys of a tile
 constexpr int MIN_TILES = 4;                             // of a split: one tile per wave
@@ -495,9 +505,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     const int base = p.shared ? 0 : slot * a.T;          // first token row of the group
     const int r0 = rb * 16 * MT, r_end = min(p.group_rows, r0 + 16 * MT);
 
-    int len = p.kv_len;
-    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
+    const int len = rows_held(p, slot);
     const bool causal = a.causal && !p.shared;
     // rows of keys that a query row sees: all, or up to its own
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
@@ -766,9 +774,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     const int base = p.shared ? 0 : slot * a.T;
     const int r0 = rb * 64 * MT, r_end = min(p.group_rows, r0 + 64 * MT);
 
-    int len = p.kv_len;
-    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
+    const int len = rows_held(p, slot);
     const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int tiles = (n_max + KT2 - 1) / KT2;
@@ -1002,9 +1008,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const int base = p.shared ? 0 : slot * a.T;
     const int r0 = rb * 256, r_end = min(p.group_rows, r0 + 256);
 
-    int len = p.kv_len;
-    if (!p.shared && p.kv_lens) len = p.kv_lens[slot];
-    len = __builtin_amdgcn_readfirstlane(max(0, min(len, p.c.rows)));
+    const int len = rows_held(p, slot);
     const bool causal = a.causal && !p.shared;
     const int n_max = causal ? max(0, min(len, len - a.T + (r_end - 1) / a.GH + 1)) : len;
     const int n_min = causal ? len - a.T + r0 / a.GH + 1 : len;
@@ -1548,7 +1552,7 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
                          "scale=%g (finite, above 0)", B, cache->slots, T, H, G, ldq, ldo, kv_max, scale);
         return SEEDMI_E_SHAPE;
     }
-    if (!kv_lens_i32 && (kv_len < 0 || kv_len > cache->rows)) {
+    if (kv_len < 0 || kv_len > cache->rows) {
         seedmi_set_error("seedmi_kv_attention: kv_len %d of a cache of %d rows", kv_len, cache->rows);
         return SEEDMI_E_SHAPE;
     }

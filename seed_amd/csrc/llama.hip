@@ -1833,9 +1833,18 @@ extern "C" int seedmi_llama_forward_ex(const seedmi_llama_weights_t* w, const vo
                                    workspace, workspace_bytes, stream);
 }
 
+// cache handles in place of the layers' static caches (seedmi_llama_forward_kv)
+struct KvPath {
+    const seedmi_kv_cache_t *kv, *prefix;
+    int prefix_len, past_max;
+    const void* past_lens;
+    void* ws;
+    size_t ws_bytes;
+};
 static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i64, const void* inputs_embeds, const void* pos_i64,
                               int batch, int T, int past_len, const void* past_len_dev, int past_stride, int last_only,
-                              void* logits, int ldl, void* hidden_states, void* workspace, size_t workspace_bytes, void* stream);
+                              void* logits, int ldl, void* hidden_states, void* workspace, size_t workspace_bytes, void* stream,
+                              const KvPath* path = nullptr);
 
 extern "C" int seedmi_llama_forward_io(const seedmi_llama_weights_t* w, const void* ids_i64, const void* inputs_embeds,
                                        const void* pos_i64, int batch, int T, int past_len, const void* past_len_dev,
@@ -1860,7 +1869,8 @@ extern "C" int seedmi_llama_decode_slots(const seedmi_llama_weights_t* w, const 
 
 static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i64, const void* inputs_embeds, const void* pos_i64,
                               int batch, int T, int past_len, const void* past_len_dev, int past_stride, int last_only,
-                              void* logits, int ldl, void* hidden_states, void* workspace, size_t workspace_bytes, void* stream) {
+                              void* logits, int ldl, void* hidden_states, void* workspace, size_t workspace_bytes, void* stream,
+                              const KvPath* path) {
     if (!w || (!ids_i64 && !inputs_embeds) || (ids_i64 && inputs_embeds) || (!pos_i64 && !past_len_dev) || !logits || batch <= 0 ||
         T <= 0) {
         seedmi_set_error("seedmi_llama_forward: null argument, both/neither of ids and inputs_embeds, or bad batch/T");
@@ -1870,11 +1880,11 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
         seedmi_set_error("seedmi_llama_forward_io: hidden_states are produced for all positions (last_only must be 0)");
         return SEEDMI_E_SHAPE;
     }
-    if (past_len_dev && T != 1) {
+    if (past_len_dev && T != 1 && !path) {
         seedmi_set_error("seedmi_llama_forward_ex: a device-resident past_len is only valid for single-token decode steps");
         return SEEDMI_E_SHAPE;
     }
-    if (batch > w->batch_cap || past_len + T > w->tmax || past_len + T > w->max_pos) {
+    if (!path && (batch > w->batch_cap || past_len + T > w->tmax || past_len + T > w->max_pos)) {
         seedmi_set_error("seedmi_llama_forward: batch %d (cap %d) / length %d (cache %d, rope table %d)", batch,
                          w->batch_cap, past_len + T, w->tmax, w->max_pos);
         return SEEDMI_E_SHAPE;
@@ -1936,7 +1946,7 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
     if (fold && !fused_first) CK(seedmi_pack_activations_bf16(t.x, h, t.xn, M, h, stream));
     int mega_done = 0;
 #ifdef SEEDMI_DEVTOOLS
-    if (fold && g_decode_fused && !hidden_states)
+    if (fold && g_decode_fused && !hidden_states && !path)
         CK(decode_layers_launch(w, t, batch, pos_i64, past_len, past_len_dev, past_stride, scale, (hipStream_t)stream, &mega_done));
 #endif
     for (int l = 0; l < w->layers && !mega_done; ++l) {
@@ -1952,7 +1962,16 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
             CK(linear(M, 3 * h, h, t.xn, h, L.qkv_w, (pk || !w->norm_folded) ? L.qkv_wp : nullptr, nullptr, 0, EPI_NONE, t.qkv, 3 * h,
                       stream, pk, 0, sk, gsk, t.gsk_bytes));
         }
-        if (T == 1 && g_decode_fused) {
+        if (path) {
+            // append and attention by cache handle; the attention's rows are row-major, so decode steps repack them for the o_proj GEMM
+            // (xn is free here: the q/k/v GEMM has consumed it, the o_proj GEMM writes it next)
+            bf16_t* const rows = pk ? t.xn : t.att;
+            CK(seedmi_kv_append(&path->kv[l], t.qkv, 3 * h, nullptr, path->prefix_len, w->cos_t, w->sin_t, w->max_pos, t.q, h, batch, T, H, 0,
+                                path->past_lens, stream));
+            CK(seedmi_kv_attention(&path->kv[l], path->prefix_len ? &path->prefix[l] : nullptr, path->prefix_len, t.q, h, rows, h, batch, T, H, T,
+                                   path->past_lens, path->past_max + T, scale, 1, path->ws, path->ws_bytes, stream));
+            if (pk) CK(seedmi_pack_activations_bf16(rows, h, t.att, M, h, stream));
+        } else if (T == 1 && g_decode_fused) {
             // RoPE + cache append + attention in one launch (bit-identical to the two-kernel form below)
             CK(decode_attention_launch(t.qkv, 3 * h, past_len_dev ? nullptr : pos_i64, w->cos_t, w->sin_t, L.k_cache, L.v_cache, t.att, h,
                                        batch, H, hd, w->tmax, past_len, scale, pk, past_len_dev, past_stride, w->max_pos, stream));
@@ -1997,4 +2016,29 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
                   nullptr, gsk, t.gsk_bytes));
     }
     return SEEDMI_OK;
+}
+
+extern "C" int seedmi_llama_forward_kv(const seedmi_llama_weights_t* w, const seedmi_kv_cache_t* kv, const seedmi_kv_cache_t* prefix, int prefix_len,
+                                       const void* ids_i64, int batch, int T, const void* past_lens_i32, int past_max, int last_only, void* logits,
+                                       int ldl, void* attn_workspace, size_t attn_workspace_bytes, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+    if (!w || !kv || !ids_i64 || !past_lens_i32 || batch <= 0 || T <= 0 || past_max < 0 || prefix_len < 0 || (prefix_len > 0 && !prefix)) {
+        seedmi_set_error("seedmi_llama_forward_kv: null argument, bad batch / T / past_max, or prefix_len without a prefix");
+        return SEEDMI_E_SHAPE;
+    }
+    for (int l = 0; l < w->layers; ++l) {
+        if (kv[l].kv_heads != w->heads || kv[l].head_dim != w->hidden / w->heads || kv[l].slots < batch || kv[l].rows < 1) {
+            seedmi_set_error("seedmi_llama_forward_kv: layer %d's cache has %d heads of %d, %d slots; the model %d heads of %d, batch %d", l,
+                             kv[l].kv_heads, kv[l].head_dim, kv[l].slots, w->heads, w->hidden / w->heads, batch);
+            return SEEDMI_E_SHAPE;
+        }
+        if ((long long)past_max + T > kv[l].rows || (long long)prefix_len + past_max + T > w->max_pos) {
+            seedmi_set_error("seedmi_llama_forward_kv: %d + %d rows of a cache of %d, behind a prefix of %d (rope table %d)", past_max, T, kv[l].rows,
+                             prefix_len, w->max_pos);
+            return SEEDMI_E_SHAPE;
+        }
+    }
+    const KvPath path = {kv, prefix, prefix_len, past_max, past_lens_i32, attn_workspace, attn_workspace_bytes};
+    return llama_forward_impl(w, ids_i64, nullptr, nullptr, batch, T, past_max, past_lens_i32, 1, last_only, logits, ldl, nullptr, workspace,
+                              workspace_bytes, stream, &path);
 }

@@ -195,6 +195,24 @@ class KVCache:
         return k_out, v_out
 
 
+class LayerCaches:
+    """One cache per decoder layer, alike in shape and format: what ``LlamaEngine.forward_kv`` appends to and attends over."""
+
+    def __init__(self, caches):
+        caches = list(caches)
+        first = caches[0]
+        alike = lambda c: (c.slots, c.kv_heads, c.rows, c.head_dim, c.format, c.dtype, c.device)  # noqa: E731
+        if any(alike(c) != alike(first) for c in caches):
+            raise ValueError("LayerCaches: the layers' caches must be alike")
+        self.layers = caches
+        self.slots, self.rows, self.format, self.dtype, self.device = first.slots, first.rows, first.format, first.dtype, first.device
+        self.array = (L.KVCacheStruct * len(caches))(*(c.struct for c in caches))
+
+    def slot(self, s: int) -> "LayerCaches":
+        """One slot of every layer (a shared prompt, a conversation prefilled alone)."""
+        return LayerCaches(c.slot(s) for c in self.layers)
+
+
 class KVAttention:
     """Attention of ``heads`` query heads over a ``KVCache``, ``tokens`` query rows per slot, made once and called every step.
 
@@ -225,14 +243,16 @@ class KVAttention:
         self._ws = (self.workspace.data_ptr(), need) if need else (None, 0)
         self._fn, self._rows, self._cols = cache.lib.seedmi_kv_attention, self.slots * tokens, heads * cache.head_dim
 
-    def __call__(self, q: torch.Tensor, kv_len: Lengths, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def __call__(self, q: torch.Tensor, kv_len: Lengths, out: Optional[torch.Tensor] = None, plus: int = 0) -> torch.Tensor:
         """q [slots * tokens, heads * head_dim] -> out of the same shape; ``kv_len``: rows each slot holds, the query rows' own included
-        (an int, or an int32 tensor with one entry per slot; 0 for an idle slot).  Queries that see nothing get zeros."""
+        (an int, or an int32 tensor with one entry per slot; 0 or less for an idle slot).  ``plus`` is added to a tensor's entries that are not
+        negative: ``attention(q, past, plus=T)`` takes the lengths that ``append`` took.  Queries that see nothing get zeros."""
         c, cols, rows = self.cache, self._cols, self._rows
         ldq = c._rows_of("KVAttention", q, cols)
         if q.size(0) != rows:
             raise ValueError(f"KVAttention: {q.size(0)} query rows, made for {self.slots} slots of {self.tokens}")
         n, lens = c._lengths("KVAttention", kv_len, self.slots)
+        n += plus
         if out is None:
             out, ldo = torch.empty((rows, cols), dtype=c.dtype, device=c.device), cols
         else:

@@ -135,6 +135,8 @@ SIGNATURES = {
     "seedmi_kv_attention_workspace_init": (_i, [_vp, C.c_size_t, _vp]),
     "seedmi_kv_attention": (_i, [C.POINTER(KVCacheStruct), C.POINTER(KVCacheStruct), _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _i,
                                  C.c_float, _i, _vp, C.c_size_t, _vp]),
+    "seedmi_llama_forward_kv": (_i, [C.POINTER(LlamaWeights), C.POINTER(KVCacheStruct), C.POINTER(KVCacheStruct), _i, _vp, _i, _i, _vp, _i, _i,
+                                     _vp, _i, _vp, C.c_size_t, _vp, C.c_size_t, _vp]),
     "seedmi_preprocess_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i]),
     "seedmi_preprocess_image_u8": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, C.POINTER(C.c_float), C.POINTER(C.c_float),
                                         _vp, _i, _vp, _vp, C.c_size_t, _vp]),

@@ -20,6 +20,7 @@ import torch
 
 from . import lib as L
 from .config import LlamaConfig
+from .kv_cache import KVCache, LayerCaches
 
 
 def _round_up(x, m):
@@ -55,6 +56,8 @@ class LlamaEngine:
         self._keep = []
         self._ws = None
         self._ws_key = (0, 0)
+        self._kv_ws = None                     # forward_kv's attention workspace
+        self._kv_refs = []                     # workspaces that forward_kv has used: a call captured into a graph replays on them
         self.past_len = 0
         self.cache_generation = 0              # bumped by resize_cache: consumers that baked cache addresses in compare it
         self._pack(state_dict)
@@ -199,6 +202,46 @@ class LlamaEngine:
         if hidden is not None:
             hidden_states_out.extend(hidden[i] for i in range(cfg.layers + 1))
         return logits.view(B, Tout, self.vocab_pad)[:, :, :cfg.vocab]
+
+    # ------------------------------------------------------------------ caches by handle
+    def new_kv(self, slots: int, rows: int, format: str = "mx8") -> LayerCaches:
+        """Caches for ``forward_kv``, one per layer: ``slots`` conversations of up to ``rows`` positions, in the 8-bit block format ("mx8", half
+        the bytes) or in 16 bits ("16")."""
+        return LayerCaches(KVCache.new(slots, self.cfg.heads, rows, self.cfg.head_dim, format, self.dtype, self.device)
+                           for _ in range(self.cfg.layers))
+
+    def forward_kv(self, input_ids: torch.Tensor, kv: LayerCaches, past: torch.Tensor, past_max: int, prefix: Optional[LayerCaches] = None,
+                   prefix_len: int = 0, last_only: bool = False) -> torch.Tensor:
+        """``forward`` over caches of the caller's: input_ids int64 [B,T], slot b of ``kv`` holds ``past[b]`` positions (int32 on the device,
+        at most ``past_max``; negative: idle, its logits mean nothing) and T more are appended.  ``prefix`` / ``prefix_len``: positions in
+        front that all slots share, held once (``new_kv(1, n)``, filled by a call of its own).  Returns logits [B, T or 1, vocab].  The
+        caller advances ``past``; a captured call replays as it grows, up to ``past_max``."""
+        if input_ids.dim() != 2:
+            raise ValueError("You have to specify input_ids of shape [batch, seq]")
+        B, T = input_ids.shape
+        if len(kv.layers) != self.cfg.layers or kv.dtype != self.dtype or kv.device != self.device:
+            raise ValueError(f"forward_kv: caches of {len(kv.layers)} layers, {kv.dtype} on {kv.device}; the model has {self.cfg.layers}, "
+                             f"{self.dtype} on {self.device}")
+        if prefix_len and (prefix is None or len(prefix.layers) != self.cfg.layers or prefix.dtype != self.dtype or prefix.device != self.device):
+            raise ValueError("forward_kv: prefix_len without a prefix of the model's layers, type and device")
+        if past.dtype != torch.int32 or past.device != self.device or past.numel() != B or not past.is_contiguous():
+            raise ValueError(f"forward_kv: past must be {B} contiguous int32 on {self.device}")
+        input_ids = input_ids.to(device=self.device, dtype=torch.int64).contiguous()
+        logits = torch.empty(B * (1 if last_only else T), self.vocab_pad, dtype=self.dtype, device=self.device)
+        ws = self._workspace(B, T)
+        need = self.lib.seedmi_kv_attention_workspace_bytes(kv.array, B, T, self.cfg.heads, past_max + T, prefix_len)
+        with torch.cuda.device(self.device):
+            if need > (0 if self._kv_ws is None else self._kv_ws.numel()):
+                self._kv_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+                L.check(self.lib.seedmi_kv_attention_workspace_init(L.ptr(self._kv_ws), need, L.stream_ptr()), "seedmi_kv_attention_workspace_init",
+                        self.lib)
+            if not self._kv_refs or self._kv_refs[-1][0] is not ws or self._kv_refs[-1][1] is not self._kv_ws:
+                self._kv_refs.append((ws, self._kv_ws))
+            rc = self.lib.seedmi_llama_forward_kv(C.byref(self.w), kv.array, prefix.array if prefix_len else None, prefix_len, L.ptr(input_ids), B, T,
+                                                  L.ptr(past), past_max, 1 if last_only else 0, L.ptr(logits), self.vocab_pad, L.ptr(self._kv_ws),
+                                                  0 if self._kv_ws is None else self._kv_ws.numel(), L.ptr(ws), ws.numel(), L.stream_ptr())
+        L.check(rc, "seedmi_llama_forward_kv", self.lib)
+        return logits.view(B, -1, self.vocab_pad)[:, :, :self.cfg.vocab]
 
     def resize_cache(self, batch_cap: Optional[int] = None, tmax: Optional[int] = None):
         """Grow (or shrink) the static KV cache in place of a rebuild: the packed weights stay where they are, the cached

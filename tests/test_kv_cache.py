@@ -112,6 +112,20 @@ def test_workspace_init_refuses():
     assert init(None, 8192, None) == E_ALIGN and init(FAKE, 4095, None) == E_ALIGN and init(FAKE + 128, 8192, None) == E_ALIGN
 
 
+def test_llama_forward_kv_refuses():
+    f = L.load().seedmi_llama_forward_kv
+    w = L.LlamaWeights()
+    w.hidden, w.layers, w.heads, w.max_pos = 256, 1, 2, 64
+    kv = (L.KVCacheStruct * 1)(_handle())
+    args = dict(w=C.byref(w), kv=kv, prefix=None, plen=0, ids=FAKE, batch=4, T=2, past=FAKE, past_max=8, last=0, logits=FAKE, ldl=64, aws=None, ab=0,
+                ws=FAKE, wb=0)
+    for bad in (dict(w=None), dict(kv=None), dict(ids=None), dict(past=None), dict(batch=0), dict(batch=5), dict(T=0), dict(past_max=-1),
+                dict(past_max=63), dict(plen=1), dict(plen=-1), dict(plen=60, prefix=kv)):
+        assert f(*dict(args, **bad).values(), None) == E_SHAPE, bad
+    w.heads = 4
+    assert f(*args.values(), None) == E_SHAPE                                      # another number of heads than the caches
+
+
 def test_layout_of_the_handle(tmp_path):
     """The struct of include/seedmi.h, compiled as plain C, against its ctypes mirror."""
     fields = [f for f, _ in L.KVCacheStruct._fields_]
