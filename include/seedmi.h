@@ -283,7 +283,7 @@ int seedmi_gemm_skinny_packed_bf16(int M, int N, int K, const void* A, int lda, 
  * ((s * slot_rows + h * head_rows) + r) * head_dim of k / v and, for MX8, at byte ((s * slot_rows + h * head_rows) + r) * head_dim / 32 of
  * k_scale / v_scale.  Rows 0 .. rows - 1 (at most 2^22) of every (slot, head) belong to the caller's allocation; nothing outside them is touched.
  * A contiguous [slots][kv_heads][rows][head_dim] cache has head_rows = rows and slot_rows = kv_heads * rows.  head_dim is 64 or 128.
- * k and v are 16-byte aligned, k_scale and v_scale 4-byte aligned (NULL for 16BIT).
+ * k and v are 16-byte aligned, k_scale and v_scale to a row's head_dim / 32 bytes (NULL for 16BIT).
  * MX8: a = the largest finite magnitude of a block of 32; e = the smallest integer >= -126 with a <= 448 * 2^e; scale byte = e + 127; an
  * element x is stored as e4m3(x / 2^e), to nearest even (off by at most 2^-4 of x, or 2^-10 * 2^e for the smallest).  Infinities and NaN
  * are stored as NaN and do not enter a; magnitudes above 1.875 * 2^127 (fp16 build: 1.875 * 2^15) are stored as that, so that every finite

@@ -1321,8 +1321,8 @@ int check_cache(const char* who, const seedmi_kv_cache_t* c, KvView* v) {
         seedmi_set_error("%s: scale bytes belong to an MX8 cache and to no other", who);
         return SEEDMI_E_SHAPE;
     }
-    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3)) {
-        seedmi_set_error("%s: k / v must be 16-byte aligned, k_scale / v_scale 4-byte aligned", who);
+    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & (unsigned)(c->head_dim / 32 - 1))) {
+        seedmi_set_error("%s: k / v must be 16-byte aligned, k_scale / v_scale aligned to a row's head_dim / 32 bytes", who);
         return SEEDMI_E_ALIGN;
     }
     *v = {(char*)c->k, (char*)c->v, (uint8_t*)c->k_scale, (uint8_t*)c->v_scale, c->slot_rows, c->head_rows, c->rows, c->kv_heads};
@@ -1387,7 +1387,7 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
         seedmi_set_error("seedmi_kv_read: the rows of a 16-bit cache are what they are: only MX8 caches are read back");
         return SEEDMI_E_DTYPE;
     }
-    if ((!k_out && !v_out) || B <= 0 || B > cache->slots || n < 0 || (!starts_i32 && (start < 0 || (long long)start + n > cache->rows))) {
+    if ((n > 0 && !k_out && !v_out) || B <= 0 || B > cache->slots || n < 0 || (!starts_i32 && (start < 0 || (long long)start + n > cache->rows))) {
         seedmi_set_error("seedmi_kv_read: no output, B=%d (slots %d), or rows %d .. + %d of a cache of %d", B, cache->slots, start, n, cache->rows);
         return SEEDMI_E_SHAPE;
     }
@@ -1407,7 +1407,7 @@ extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void*
 }
 
 // How a call is cut: a pass over the slots' own rows and, with a prefix, one over the prefix; row blocks and key ranges of each.
-struct KvPass { int groups, group_rows, block_rows, row_blocks, splits, per_split; unsigned blocks; };
+struct KvPass { int groups, group_rows, block_rows, row_blocks, splits, per_split; long long blocks; };
 struct KvPlan {
     KvPass own, pre;
     int parts, units, unit_rows;                         // units > 0: joined in place, by the last workgroup of each unit
@@ -1434,7 +1434,7 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     p.splits = (int)(s < 1 ? 1 : s);
     p.per_split = (int)((tiles + p.splits - 1) / p.splits);
     if (p.per_split < MIN_TILES) p.per_split = MIN_TILES;
-    p.blocks = ((unsigned)p.groups * p.splits + 7) / 8 * 8 * p.row_blocks;
+    p.blocks = ((long long)p.groups * p.splits + 7) / 8 * 8 * p.row_blocks;
     return p;
 }
 
@@ -1451,6 +1451,8 @@ static int make_plan(const seedmi_kv_cache_t* c, int B, int T, int H, int kv_max
     pl->own = plan_pass(B * c->kv_heads, (long long)T * GH, keys);
     pl->pre = prefix_len ? plan_pass(c->kv_heads, (long long)B * T * GH, prefix_len) : KvPass{};
     pl->parts = pl->own.splits + pl->pre.splits;
+    // a launch has fewer than 2^32 threads
+    if ((pl->own.blocks + pl->pre.blocks) * 512 > UINT_MAX || (pl->parts > 1 && pl->rows * (c->head_dim / 4) * 8 > UINT_MAX)) return -1;
     pl->units = pl->unit_rows = 0;
     pl->unit_blocks = 0;
     if (pl->parts > 1 && pl->own.block_rows <= 32 && (!prefix_len || pl->pre.block_rows == pl->own.block_rows)) {
@@ -1505,20 +1507,20 @@ template <int HD, bool MX>
 static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, const KvPlan& pl, int prefix_len, int kv_len, const int* kv_lens,
                              hipStream_t s) {
     auto set = [](AttnPass& x, const KvView& v, const KvPass& p, int shared, int part0, int len, const int* lens) {
-        x = {v, lens, len, shared, p.groups, p.group_rows, p.row_blocks, p.splits, part0, p.per_split, p.blocks};
+        x = {v, lens, len, shared, p.groups, p.group_rows, p.row_blocks, p.splits, part0, p.per_split, (unsigned)p.blocks};
     };
     if (!prefix_len) {
         set(a.pass[0], own, pl.own, 0, 0, kv_len, kv_lens);
-        launch_blocks<HD, MX>(a, pl.own.block_rows, pl.own.blocks, s);
+        launch_blocks<HD, MX>(a, pl.own.block_rows, (unsigned)pl.own.blocks, s);
     } else {
         set(a.pass[0], pre, pl.pre, 1, 0, prefix_len, nullptr);
         set(a.pass[1], own, pl.own, 0, pl.pre.splits, kv_len, kv_lens);
         if (pl.pre.block_rows == pl.own.block_rows) {    // one kernel for both: one launch
-            launch_blocks<HD, MX>(a, pl.own.block_rows, pl.pre.blocks + pl.own.blocks, s);
+            launch_blocks<HD, MX>(a, pl.own.block_rows, (unsigned)(pl.pre.blocks + pl.own.blocks), s);
         } else {
-            launch_blocks<HD, MX>(a, pl.pre.block_rows, pl.pre.blocks, s);
+            launch_blocks<HD, MX>(a, pl.pre.block_rows, (unsigned)pl.pre.blocks, s);
             a.pass[0] = a.pass[1];
-            launch_blocks<HD, MX>(a, pl.own.block_rows, pl.own.blocks, s);
+            launch_blocks<HD, MX>(a, pl.own.block_rows, (unsigned)pl.own.blocks, s);
         }
     }
     if (pl.parts > 1 && !pl.units) {
@@ -1562,7 +1564,7 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
     }
     KvPlan pl;
     if (make_plan(cache, B, T, H, kv_max, prefix_len, &pl)) {
-        seedmi_set_error("seedmi_kv_attention: B * T * H = %lld: at most 2^31 - 1", (long long)B * T * H);
+        seedmi_set_error("seedmi_kv_attention: B * T * H = %lld rows need more threads than a launch has (2^32)", (long long)B * T * H);
         return SEEDMI_E_SHAPE;
     }
     if (pl.bytes && (!workspace || workspace_bytes < pl.bytes || ((uintptr_t)workspace & 255))) {

@@ -200,6 +200,8 @@ class LayerCaches:
 
     def __init__(self, caches):
         caches = list(caches)
+        if not caches:
+            raise ValueError("LayerCaches: no layers")
         first = caches[0]
         alike = lambda c: (c.slots, c.kv_heads, c.rows, c.head_dim, c.format, c.dtype, c.device)  # noqa: E731
         if any(alike(c) != alike(first) for c in caches):
@@ -240,6 +242,9 @@ class KVAttention:
         if need:
             _call(cache.index, cache.lib.seedmi_kv_attention_workspace_init, "seedmi_kv_attention_workspace_init", cache.lib,
                   self.workspace.data_ptr(), need)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(cache.device).synchronize()              # ready for a first call on any stream
+        self._home = _current_stream(cache.index)
         self._ws = (self.workspace.data_ptr(), need) if need else (None, 0)
         self._fn, self._rows, self._cols = cache.lib.seedmi_kv_attention, self.slots * tokens, heads * cache.head_dim
 
@@ -259,6 +264,8 @@ class KVAttention:
             ldo = c._rows_of("KVAttention (out)", out, cols)
             if out.size(0) != rows:
                 raise ValueError(f"KVAttention: out has {out.size(0)} rows, not {rows}")
+        if self.workspace is not None and _current_stream(c.index) != self._home:
+            self.workspace.record_stream(torch.cuda.current_stream(c.device))      # (freed memory is not handed on while that stream uses it)
         _call(c.index, self._fn, "seedmi_kv_attention", c.lib, c._ref, self._pref, self.prefix_len, q.data_ptr(), ldq, out.data_ptr(), ldo, self.slots,
               self.tokens, self.heads, n, lens, self.kv_max, self.scale, self.causal, self._ws[0], self._ws[1])
         return out

@@ -437,6 +437,41 @@ def test_transposed_layout_and_one_slot_views():
     _check(one, q[:5], per_slot[1:2], None, 4, G, 5, 1.0 / math.sqrt(D), True)
 
 
+def test_odd_rows_of_64_values_and_slot_views():
+    """33 rows of 64: scale rows of two bytes at every second address, slots alone as caches of their own, all written, read and attended to."""
+    B, G, D, rows = 3, 1, 64, 33
+    cache = _poisoned(B, G, rows, D, "mx8", BF)
+    per_slot = [_fill(cache, b, rows, 7 * b + 1) for b in range(B)]
+    for b in range(B):
+        one = cache.slot(b)
+        k, v = one.read(0, rows)
+        assert torch.equal(k[0].cpu().double(), per_slot[b][0]) and torch.equal(v[0].cpu().double(), per_slot[b][1])
+        for T in (1, 30, 33):
+            q = _rand((T, 2 * D), BF, 6).cuda()
+            _check(KVAttention(one, heads=2, tokens=T)(q, rows), q, per_slot[b:b + 1], None, 2, G, T, 1.0 / math.sqrt(D), True)
+    x = _rand((1, 4 * D), BF, 8)
+    cos, sin = (t.cuda() for t in _tables(64, D, BF))
+    cache.slot(1).append(x.cuda(), cos, sin, 32, heads=2)
+    code, byte = R.mx_encode(x.view(4, D)[3], R.top(BF))
+    assert torch.equal(cache.v[1, 0, 32].cpu(), code) and torch.equal(cache.v_scale[1, 0, 32].cpu(), byte)
+    k, v = cache.read(0, 0)
+    assert k.shape == (B, G, 0, D) and v.shape == k.shape
+
+
+def test_lengths_plus_the_new_rows():
+    """plus = T on the lengths before the append: the same bits as lengths that count the new rows; idle slots stay idle."""
+    H, D = 2, 128
+    cache = _poisoned(3, H, 80, D, "mx8", BF)
+    for b in range(3):
+        _fill(cache, b, 80, 7 * b + 1)
+    for T in (1, 4, 70):
+        q = _rand((3 * T, H * D), BF, 6).cuda()
+        attn = KVAttention(cache, heads=H, tokens=T)
+        a = attn(q, torch.tensor([5, -1, 80 - T], dtype=torch.int32).cuda(), plus=T)
+        b = attn(q, torch.tensor([5 + T, 0, 80], dtype=torch.int32).cuda())
+        assert torch.equal(a, b) and (a.view(3, T, -1)[1] == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ streams, graphs, the operators together
 def test_a_captured_step_replays_with_new_lengths():
     """append + attention of one token in a graph whose lengths live on the device, replayed between eager work; a second captured object

@@ -47,6 +47,7 @@ def _attend(h, p=None, **kw):
                                       (dict(rows=(1 << 22) + 1), E_SHAPE),
                                       (dict(head_dim=96), E_SHAPE), (dict(format=2), E_DTYPE), (dict(k_scale=None), E_SHAPE),
                                       (dict(format=L.KV_16BIT), E_SHAPE), (dict(v=FAKE + 8), E_ALIGN), (dict(v_scale=FAKE + 2), E_ALIGN),
+                                      (dict(v_scale=FAKE + 1, head_dim=64), E_ALIGN),
                                       (dict(head_rows=-1), E_SHAPE), (dict(slot_rows=-64), E_SHAPE)])
 def test_bad_handles_are_refused(call, bad, code):
     assert call(_handle(**bad)) == code
@@ -76,14 +77,15 @@ def test_read_refuses(kw, code):
 
 
 def test_read_of_no_rows_is_nothing_and_16_bit_rows_are_refused():
-    assert _read(_handle(), n=0) == 0
+    assert _read(_handle(), n=0) == 0 and _read(_handle(), n=0, k=None, v=None) == 0
     assert _read(_handle(format=L.KV_16BIT, k_scale=None, v_scale=None)) == E_DTYPE
 
 
 @pytest.mark.parametrize("kw,code", [(dict(B=5), E_SHAPE), (dict(T=0), E_SHAPE), (dict(H=3), E_SHAPE), (dict(kv_len=65), E_SHAPE),
                                      (dict(kv_len=-1), E_SHAPE), (dict(ldq=504), E_SHAPE), (dict(ldo=504), E_SHAPE), (dict(ldo=516), E_ALIGN),
                                      (dict(q=FAKE + 8), E_ALIGN), (dict(kv_max=-1), E_SHAPE), (dict(scale=float("nan")), E_SHAPE),
-                                     (dict(plen=1), E_SHAPE), (dict(plen=-1), E_SHAPE), (dict(T=1 << 28), E_SHAPE)])
+                                     (dict(plen=1), E_SHAPE), (dict(plen=-1), E_SHAPE), (dict(T=1 << 28), E_SHAPE),
+                                     (dict(kv_len=65, lens=FAKE), E_SHAPE)])
 def test_attention_refuses(kw, code):
     assert _attend(_handle(), **kw) == code
 
@@ -92,6 +94,11 @@ def test_attention_refuses_a_prefix_that_does_not_fit():
     ok = dict(slots=1)
     for bad in (dict(head_dim=64), dict(kv_heads=1), dict(format=L.KV_16BIT, k_scale=None, v_scale=None), dict(rows=31)):
         assert _attend(_handle(), _handle(**ok, **bad), plen=32) == E_SHAPE
+
+
+def test_attention_refuses_more_threads_than_a_launch_has():
+    h = _handle(slots=1 << 24)
+    assert _attend(h, B=1 << 24) == E_SHAPE and "2^32" in L.load().seedmi_last_error().decode()
 
 
 def test_attention_refuses_a_short_workspace():
