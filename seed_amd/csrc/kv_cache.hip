@@ -514,6 +514,14 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     const int per = max((tiles + p.splits - 1) / p.splits, p.per_split);
     const int t_begin = split * per, t_end = min(tiles, t_begin + per);
 
+    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
+    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
+    Tile<HD, MX> t;                                      // (the first tile is on its way while the queries are fetched)
+    if (t_begin + wave < t_end) {
+        load_v(t, rows, (t_begin + wave) * KT, lane);
+        load_k(t, rows, (t_begin + wave) * KT, lane);
+    }
+
     bf16x8 qf[MT][KS];
     int seen[MT];
     float m[MT], l[MT];
@@ -536,16 +544,9 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
-    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     char* lds = sm + wave * VBYTES;
 
     arrived(qf);
-    Tile<HD, MX> t;
-    if (t_begin + wave < t_end) {
-        load_v(t, rows, (t_begin + wave) * KT, lane);
-        load_k(t, rows, (t_begin + wave) * KT, lane);
-    }
 #pragma unroll 1
     for (int tile = t_begin + wave; tile < t_end; tile += 4) {
         const int key0 = tile * KT, next0 = (tile + 4 < t_end ? tile + 4 : tiles) * KT;    // (behind the last row: nothing is fetched)
@@ -785,6 +786,12 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
     const int wave_max = w0 >= r_end ? 0 : causal ? len - a.T + w1 / a.GH + 1 : len;
     const int wave_min = w0 >= r_end ? 0 : causal ? len - a.T + w0 / a.GH + 1 : len;
 
+    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
+    using S = Stage<HD, MX>;
+    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
+    S st;                                                // (the first tile is on its way while the queries are fetched)
+    if (t_begin < t_end) stage_load(st, rows, t_begin * KT2, tid);
+
     bf16x8 qf[MT][KS];
     int seen[MT];
     float m[MT], l[MT];
@@ -806,13 +813,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
-    using S = Stage<HD, MX>;
-    const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     arrived(qf);
-    S st;
     if (t_begin < t_end) {
-        stage_load(st, rows, t_begin * KT2, tid);
         stage_store(st, sm, sm + 2 * KB, tid);
         stage_load(st, rows, (t_begin + 1 < t_end ? t_begin + 1 : tiles) * KT2, tid);
     }
@@ -1024,29 +1026,12 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const bool on = r < r_end;
     const int token = base + (on ? r / a.GH : 0), head = kvh * a.GH + (on ? r % a.GH : 0);
     const int seen = on ? (causal ? len - a.T + r / a.GH + 1 : len) : 0;
-    bf16x8 qf[1][KS];
-    {
-        const bf16_t* qp = a.q + (size_t)token * a.ldq + head * HD + 8 * h;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (on) v = *(const uint4*)(qp + 16 * ks);
-            qf[0][ks] = __builtin_bit_cast(bf16x8, v);
-        }
-    }
-    float m = -INFINITY, l = 0.f;
-    f32x16 o[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int d = 0; d < 16; ++d) o[i][d] = 0.f;
     const long long row0 = (p.shared ? 0ll : (long long)slot * p.c.slot_rows) + (long long)kvh * p.c.head_rows;
     using S = HalfStage<HD, MX>;
     const RowBuffers rows = row_buffers<HD, MX>(p.c, row0, n_max);
     const int srow = 32 * half + ht / S::LPR, schunk = ht % S::LPR;      // the thread's first row of a tile and its 16-byte piece of it
     const bool stages = 32 * S::LPR >= 256 || ht < 32 * S::LPR;
 
-    arrived(qf);
     constexpr int KP = k_at<HD>(1, 0), VP = w_at<HD>(1, 0);              // row pitches of the images
     S st;                                                // (a second set, requested two tiles ahead: no faster)
     // tiles from n on: behind the last row, nothing is fetched
@@ -1091,16 +1076,39 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     auto partial_tile = [&](int t) { return (t0 + t + 1) * KT2 > n_min; };               // some row of the block does not see all of it
     auto vraw = [&](int t) { return partial_tile(t) ? sm + 2 * KB + (2 + (t & 1)) * VB : nullptr; };
 
+    // the tiles staged ahead of the first phase (half 1 is one vector phase ahead) and the queries are requested together
+    S first;
     if (tid == 0) s_bad = 0;
-    __syncthreads();
     if (n > 0) {
-        load_rows(st.k, st.ks, rows.k, rows.ks, 0);
-        store_rows(st.k, st.ks, kbuf(0), KP, nullptr);
-        if (half) {                                      // half 1 is one vector phase ahead in its staging
+        load_rows(first.k, first.ks, rows.k, rows.ks, 0);
+        if (half) {
             load_rows(st.k, st.ks, rows.k, rows.ks, 1);
-            load_rows(st.v, st.vs, rows.v, rows.vs, 0);
+            load_rows(first.v, first.vs, rows.v, rows.vs, 0);
+        }
+    }
+    bf16x8 qf[1][KS];
+    {
+        const bf16_t* qp = a.q + (size_t)token * a.ldq + head * HD + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (on) v = *(const uint4*)(qp + 16 * ks);
+            qf[0][ks] = __builtin_bit_cast(bf16x8, v);
+        }
+    }
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[i][d] = 0.f;
+    arrived(qf);
+    __syncthreads();                                     // (s_bad is set)
+    if (n > 0) {
+        store_rows(first.k, first.ks, kbuf(0), KP, nullptr);
+        if (half) {
             store_rows(st.k, st.ks, kbuf(1), KP, nullptr);
-            store_rows(st.v, st.vs, vbuf(0), VP, vraw(0));
+            store_rows(first.v, first.vs, vbuf(0), VP, vraw(0));
         }
         load_rows(st.k, st.ks, rows.k, rows.ks, 1 + half);
         load_rows(st.v, st.vs, rows.v, rows.vs, half);
