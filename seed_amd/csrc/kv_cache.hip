@@ -1429,8 +1429,20 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     KvPass p = {};
     p.groups = groups;
     p.group_rows = (int)rows;
-    // up to 32 rows: the few-rows kernel with one or two blocks of 16; beyond: the many-rows kernel, 64 or 128 to a workgroup
+    // Rows of a block: the smallest that holds the group.  us for 8 x 40 heads x 1024 past rows, 8-bit, by the rows of a group (column: block):
+    //   rows    16    32    64   128   256        (16-bit rows: the same order, 33 - 37 us up to 64 rows)
+    //     16  21.6  22.8  27.0  33.8  50.7
+    //     32  25.8  24.5  31.8  35.4  51.6
+    //     48  32.0  34.4  34.1  44.5  53.9
+    //    100        51.4  57.6  53.5  60.1        2 x 8 heads x 8000 past rows, 96 rows: 24.5  26.7  26.5  24.2
+    //    256             100.3  93.0  93.1                                          192 rows:       37.1  37.3  33.3
+    // More than 256 rows leave a block of them partly empty; where that costs a round of workgroups in five, blocks of 128 (two to a CU):
+    // 300 rows of 320 groups 110 us against 134, of 16 groups 50 against 44.
     p.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    if (p.block_rows == 256) {
+        const long long by256 = ((rows + 255) / 256 * groups + 255) / 256, by128 = ((rows + 127) / 128 * groups + 511) / 512;
+        if (by128 * 5 < by256 * 4) p.block_rows = 128;
+    }
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     const int kt = p.block_rows <= 32 ? KT : KT2;
     const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
