@@ -14,6 +14,19 @@ namespace {
 
 constexpr int NORM_WAVES = 4;
 
+// Products rounded before they are added, where the compiler would be free to fuse one of them, and did or did not with the flags it was
+// given: ids moved in near ties.  These are the roundings that the norms have always had.
+SEEDMI_DEVINL float dot2_apart(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
+    const float x = a * b, y = c * d;
+    return x + y;
+}
+SEEDMI_DEVINL float add_square_apart(float s, float d) {
+#pragma clang fp contract(off)
+    const float q = d * d;
+    return s + q;
+}
+
 // one wave per row; row held in registers as MAXC chunks of 8 bf16 per lane
 // PACK: write the row in the decode GEMM's fragment-major activation layout (16-row tile x 32-k step = 1 KiB block in MFMA
 // lane order) so the consumer's operand loads are contiguous: chunk c of row m goes to
@@ -40,7 +53,9 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void norm_kernel(const bf16_t* __r
         for (int j = 0; j < 4; ++j) {
             v[i][2 * j] = lo_bf(w[j]);
             v[i][2 * j + 1] = hi_bf(w[j]);
-            sum += RMS ? (v[i][2 * j] * v[i][2 * j] + v[i][2 * j + 1] * v[i][2 * j + 1]) : (v[i][2 * j] + v[i][2 * j + 1]);
+            const float lo = v[i][2 * j], hi = v[i][2 * j + 1];
+            // squares rounded one by one; of the last chunk, where there are several, the first of a pair is fused (as it has always been)
+            sum += !RMS ? lo + hi : MAXC > 1 && i == MAXC - 1 ? fmaf(lo, lo, hi * hi) : dot2_apart(lo, lo, hi, hi);
         }
     }
     sum = wave_sum(sum);
@@ -56,7 +71,7 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void norm_kernel(const bf16_t* __r
             const int c = lane + 64 * i;
             if (c < nchunks) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { const float d = v[i][j] - mean; sq += d * d; }
+                for (int j = 0; j < 8; ++j) sq = add_square_apart(sq, v[i][j] - mean);
             }
         }
         sq = wave_sum(sq);
@@ -129,7 +144,7 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void row_stats_kernel(const bf16_t
         const int c = lane + 64 * i;
         if (c < nchunks) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { const float d = v[i][j] - mean; sq += d * d; }
+            for (int j = 0; j < 8; ++j) sq = add_square_apart(sq, v[i][j] - mean);
         }
     }
     sq = wave_sum(sq);
