@@ -58,7 +58,10 @@ struct KvView {                                          // seedmi_kv_cache_t as
 };
 
 // ------------------------------------------------------------------------------------------------ append
-// One thread = 8 values i .. i + 7 and their partners i + HD/2 .. of one (slot, token, head): a quad of lanes holds two whole blocks of 32.
+// y = half(half(x cos) + half(rotate_half(x) sin)); per block of 32 y: a = max |y|, e = min {e : a <= 448 2^e}, codes e4m3(y 2^-e).
+// One thread = 8 values i .. i + 7 and their partners i + HD/2 .. of one (slot, token, head): a quad of lanes holds two whole blocks of 32,
+// and the block maximum is two exchanges.  Bound by its bytes: 8 x 649 tokens of 40 heads (268 MB) take 59 us, 4.5 TB/s; a step of one or
+// 32 tokens 3 - 5 us, which is a launch.
 template <int HD, bool MX>
 __global__ __launch_bounds__(256) void kv_append_kernel(const KvView c, const bf16_t* __restrict__ qkv, int ldqkv,
                                                         const long long* __restrict__ pos_ids, int pos_base,
@@ -153,7 +156,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvView c, const bf
 }
 
 // ------------------------------------------------------------------------------------------------ read back
-// One thread = 16 values: 16 code bytes in, 32 bytes out.  blockIdx.y: keys / values.
+// One thread = 16 values: 16 code bytes in, 32 bytes out.  blockIdx.y: keys / values.  Bound by its bytes: 4 x 8191 rows of 32 heads (814 MB)
+// take 133 us, 6.1 TB/s (a copy of a gigabyte reaches 5.1 on this card, a read-only stream 7.0).
 template <int HD>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, int B, int n,
                                                       int start, const int* __restrict__ starts) {
@@ -480,8 +484,12 @@ SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh,
 }
 
 // ---- few query rows per group (decode, drafted tokens, a shared prefix): bound by the bytes of the cache.
+// Bytes: 2 rows of HD values per key and key head, once; 4 HD flops per (row, key) are far below what they cost up to some 100 rows.
+// 32 x 32 heads: 4096 rows each 186 us (8-bit, 6.0 TB/s) / 356 us (16-bit, 6.0); slots of different lengths up to 2048
+// rows 68 us (5.2); 4 x 8 heads of 23 - 65 thousand rows 82 us (4.6, with the parts' join); one conversation of 700 rows 8.3 us, latency.
 // Workgroup = (group, block of 16 MT rows, key range); its 4 waves take the range's tiles in turn, each with a running softmax of its own,
-// and join at the end.  S^T = K Q^T (keys are the MFMA's rows: K fragments come straight from memory, one tile ahead in registers), so a
+// and join at the end (eight waves: 4 slots of 65 thousand rows 85 -> 81 us, one short conversation 8.3 -> 9.2).
+// S^T = K Q^T (keys are the MFMA's rows: K fragments come straight from memory, one tile ahead in registers), so a
 // lane's scores are keys 4 g + r of its query li, which is the layout the P^T operand of O^T = V^T P^T needs: P never leaves registers.
 // V is transposed through 8 KiB of LDS that the wave has to itself (no barrier in the loop).
 template <int HD, bool MX, int MT>
@@ -710,7 +718,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 // ---- many query rows per group (prompt chunks, a prefix that many slots share): bound by the matrix and vector pipes.
 // Workgroup = (group, block of 64 MT rows, key range), wave = 16 MT rows; 64-key tiles of K and V are widened to 16 bits once and shared
 // through a double-buffered LDS image, one barrier per tile; the next tile's bytes are in registers meanwhile, so that neither the load nor
-// the widening sits between two tiles.
+// the widening sits between two tiles.  8 x 40 heads, 100 new rows behind 549: 40 us (8-bit) / 38 us (16-bit).
 constexpr int KT2 = 64;
 
 template <int HD, bool MX>
@@ -960,6 +968,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 // values of t + h - two LDS buffers each, always written after their last reader's barrier.
 // Tiles that every row of the block sees whole take a loop without masks and case distinctions (a lone wave issues an instruction every
 // five to six cycles, scalar ones too: it is their number that counts).
+// 2 x 32 heads, 2048 new rows each in caches of up to 4001: 138 GF in 192 us, 717 TFLOP/s (both slots at 4001 rows: 238 us, 839); a plain
+// 8192^3 product of the type reaches 1284.  With one phase's work taken out (kernel at 195 us): matrix phases alone 135 us, vector phases
+// alone 162; without the requests for the next tiles 160.
+// On 16 x 16 x 32 products and one loop for all tiles the same kernel took 232 us, unphased with two workgroups per CU 244.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 SEEDMI_DEVINL f32x16 mfma_32x32x16(bf16x8 a, bf16x8 b, f32x16 c) {
 #ifdef SEEDMI_F16
@@ -1272,7 +1284,8 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 }
 
 // The parts of every row joined.  Thread = 4 channels of a row and every JW-th of its parts (few rows have many parts: a thread that walked
-// them all would wait for one memory round trip after the other); the JW partial sums meet in the LDS.
+// them all would wait for one memory round trip after the other); the JW partial sums meet in the LDS.  JW = 8 from five parts on (48 slots
+// behind a prefix, 33 parts: 61 us in all against 72 with 1), 1 below (64 K rows of two parts: 110 us in all against 136 with 8).
 template <int HD, int JW>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml, long long rows,
                                                                 int parts, int H, bf16_t* __restrict__ out, int ldo) {
@@ -1446,8 +1459,13 @@ static KvPass plan_pass(int groups, long long rows, long long keys) {
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     const int kt = p.block_rows <= 32 ? KT : KT2;
     const long long tiles = (keys + kt - 1) / kt, base = (long long)groups * p.row_blocks;
-    // One workgroup per CU, two of the 64- and 128-row ones (they share a CU).  A range has a fixed number of tiles (of the longest slot
-    // expected), so short slots have fewer; the slots take turns from range to range, so that the CUs get as many of them each.
+    // One workgroup per CU, two of the 64- and 128-row ones (they share a CU).  Few rows: between 256 and 2048 workgroups it is flat within
+    // the noise for 4 slots of up to 65 thousand rows (82 - 85 us) and slower from 2048 on for 32 slots (68 -> 73).  192 rows of 48 slots
+    // behind a prefix of 24 thousand: 62 us in 256-row blocks (75 with 128 workgroups), 76 -> 69 in 128-row ones and 79 -> 65 in 64-row ones
+    // from 256 to 512 workgroups.
+    // At least four tiles to a range (a tile per wave): one conversation 8.35 us, with two 8.76, with eight 8.88.  A range has a fixed number
+    // of tiles (of the longest slot expected), so short slots have fewer; the slots take turns from range to range, so that the CUs get as
+    // many of them each.
     const long long target = p.block_rows == 64 || p.block_rows == 128 ? 512 : 256;
     long long s = target / base;
     if (s > (tiles + MIN_TILES - 1) / MIN_TILES) s = (tiles + MIN_TILES - 1) / MIN_TILES;
@@ -1476,7 +1494,8 @@ static int make_plan(const seedmi_kv_cache_t* c, int B, int T, int H, int kv_max
     pl->units = pl->unit_rows = 0;
     pl->unit_blocks = 0;
     if (pl->parts > 1 && pl->own.block_rows <= 32 && (!prefix_len || pl->pre.block_rows == pl->own.block_rows)) {
-        // Joined in place where a unit's rows and parts are few enough for one workgroup: a second launch costs about 4 us
+        // Joined in place where a unit's rows and parts are few enough for one workgroup: a second launch costs about 3 us (one conversation
+        // of 700 rows 8.1 against 11.4 us, four samples behind a prompt 10.5 against 11.6)
         const int rows = prefix_len ? pl->pre.group_rows : pl->own.block_rows < pl->own.group_rows ? pl->own.block_rows : pl->own.group_rows;
         const long long units = prefix_len ? c->kv_heads : (long long)pl->own.groups * pl->own.row_blocks;
         if ((long long)rows * pl->parts <= 64 && units * 4 <= (long long)KV_WS_COUNTERS) {
