@@ -220,7 +220,8 @@ class KVAttention:
 
     ``prefix`` / ``prefix_len``: rows 0 .. prefix_len - 1 of a one-slot cache in front of every slot's own rows, seen whole by every query.
     ``kv_max``: the longest slot expected (default: the cache's rows); it decides how keys are split over workgroups, never the result's
-    definition.  ``causal``: query t of T sees its slot's rows up to its own; False: all of them (the keys of an encoder)."""
+    definition.  ``causal``: query t of T sees its slot's rows up to its own; False: all of them (the keys of an encoder).  The object owns
+    its workspace: calls that may run at the same time (two streams, two graphs) need an object each."""
 
     def __init__(self, cache: KVCache, heads: int, tokens: int = 1, slots: Optional[int] = None, kv_max: int = 0,
                  prefix: Optional[KVCache] = None, prefix_len: int = 0, scale: Optional[float] = None, causal: bool = True):
