@@ -73,6 +73,16 @@ SEEDMI_DEVINL void rows_to_full_lines(const unsigned (&a)[4], const unsigned (&c
 // value rounded to the 16-bit element and widened again: the point where the reference materialises a half tensor
 SEEDMI_DEVINL float rbf(float f) { return bf2f(f2bf(f)); }
 
+// An fp32 value that exists before it is rounded to the element.  The fp16 build's compiler otherwise fuses the multiplication that makes
+// it with the conversion (v_fma_mixlo_f16 rounds once: 55 of a million products differ) in one kernel and not in another, whatever the
+// contraction setting, and an image's ids then depend on its batch: the empty statement keeps the value in a register.
+SEEDMI_DEVINL float in_fp32(float f) {
+#ifdef SEEDMI_F16
+    asm("" : "+v"(f));
+#endif
+    return f;
+}
+
 // Exact-erf GELU (nn.GELU(), ACT2FN['gelu']).  erf by Abramowitz-Stegun 7.1.26 (|abs err| <= 1.5e-7, i.e. fp32-level)
 // evaluated on |z| so that 1+erf(z) for z < 0 is formed without cancellation: ~14 VALU + v_exp + v_rcp instead of the
 // ~40-instruction libm erff — the GEMM epilogue applies it to 128 values per lane and was 15 % of an fc1 tile.

@@ -401,7 +401,7 @@ SEEDMI_DEVINL void gemm_epilogue(const GemmParams& p, f32x4 (&acc)[MT][4], int m
             packed = true;
         } else if (EPI == EPI_BIAS_GELU) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = gelu_erf(rbf(v[i]));      // GELU of the half fc1 output
+            for (int i = 0; i < 16; ++i) v[i] = gelu_erf(rbf(in_fp32(v[i])));      // GELU of the half fc1 output
         } else if (EPI == EPI_BIAS_TANH) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = tanhf(rbf(v[i]));

@@ -92,8 +92,8 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void norm_kernel(const bf16_t* __r
                 float a, b2;
                 if (RMS) {
                     // x * rsqrt(var) rounded to the weight dtype BEFORE the multiply by weight (llama_xformer.py:107-113)
-                    a = lo_bf(gw[j]) * rbf(v[i][2 * j] * rstd);
-                    b2 = hi_bf(gw[j]) * rbf(v[i][2 * j + 1] * rstd);
+                    a = lo_bf(gw[j]) * rbf(in_fp32(v[i][2 * j] * rstd));
+                    b2 = hi_bf(gw[j]) * rbf(in_fp32(v[i][2 * j + 1] * rstd));
                 } else {
                     a = (v[i][2 * j] - mean) * rstd * lo_bf(gw[j]) + lo_bf(bw[j]);
                     b2 = (v[i][2 * j + 1] - mean) * rstd * hi_bf(gw[j]) + hi_bf(bw[j]);
