@@ -14,13 +14,8 @@ namespace {
 
 constexpr int NORM_WAVES = 4;
 
-// Products rounded before they are added, where the compiler would be free to fuse one of them, and did or did not with the flags it was
-// given: ids moved in near ties.  These are the roundings that the norms have always had.
-SEEDMI_DEVINL float dot2_apart(float a, float b, float c, float d) {
-#pragma clang fp contract(off)
-    const float x = a * b, y = c * d;
-    return x + y;
-}
+// The squares of a variance rounded before they are added, where the compiler would be free to fuse them, and did or did not with the flags it
+// was given: ids moved in near ties.  (Squares of 16-bit values, as in the RMS sum, are exact in fp32: there it makes no difference.)
 SEEDMI_DEVINL float add_square_apart(float s, float d) {
 #pragma clang fp contract(off)
     const float q = d * d;
@@ -53,9 +48,7 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void norm_kernel(const bf16_t* __r
         for (int j = 0; j < 4; ++j) {
             v[i][2 * j] = lo_bf(w[j]);
             v[i][2 * j + 1] = hi_bf(w[j]);
-            const float lo = v[i][2 * j], hi = v[i][2 * j + 1];
-            // squares rounded one by one; of the last chunk, where there are several, the first of a pair is fused (as it has always been)
-            sum += !RMS ? lo + hi : MAXC > 1 && i == MAXC - 1 ? fmaf(lo, lo, hi * hi) : dot2_apart(lo, lo, hi, hi);
+            sum += RMS ? (v[i][2 * j] * v[i][2 * j] + v[i][2 * j + 1] * v[i][2 * j + 1]) : (v[i][2 * j] + v[i][2 * j + 1]);
         }
     }
     sum = wave_sum(sum);
