@@ -140,7 +140,9 @@ class KVCache:
     def _batch(self, what: str, rows: int, lens: Lengths, tokens: Optional[int]):
         """Slots of a call: ``rows`` query rows are ``tokens`` of each, by default of every slot that ``lens`` lists (or of all)."""
         if tokens is not None:
-            batch = rows // tokens if tokens > 0 else 0
+            if tokens < 1 or rows % tokens:
+                raise ValueError(f"{what}: {rows} rows do not divide into slots of {tokens} tokens")
+            batch = rows // tokens
         else:
             batch = lens.numel() if isinstance(lens, torch.Tensor) else self.slots
         if batch < 1 or batch > self.slots or rows % batch:
