@@ -223,7 +223,8 @@ class KVAttention:
     ``prefix`` / ``prefix_len``: rows 0 .. prefix_len - 1 of a one-slot cache in front of every slot's own rows, seen whole by every query.
     ``kv_max``: the longest slot expected (default: the cache's rows); it decides how keys are split over workgroups, never the result's
     definition.  ``causal``: query t of T sees its slot's rows up to its own; False: all of them (the keys of an encoder).  The object owns
-    its workspace: calls that may run at the same time (two streams, two graphs) need an object each."""
+    its workspace: calls that may run at the same time (two streams, two graphs) need an object each.  It is made outside of graph captures
+    and called inside or outside of them."""
 
     def __init__(self, cache: KVCache, heads: int, tokens: int = 1, slots: Optional[int] = None, kv_max: int = 0,
                  prefix: Optional[KVCache] = None, prefix_len: int = 0, scale: Optional[float] = None, causal: bool = True):
@@ -241,12 +242,16 @@ class KVAttention:
         self.scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
         self._pref = self.prefix._ref if self.prefix_len else None
         need = cache.lib.seedmi_kv_attention_workspace_bytes(cache._ref, self.slots, tokens, heads, self.kv_max, self.prefix_len)
+        with torch.cuda.device(cache.index):
+            if need and torch.cuda.is_current_stream_capturing():
+                # (a capture records the initialisation and does not run it: calls before the first replay would join on whatever is there)
+                raise L.SeedmiError("KVAttention: this one needs a workspace, which a stream that captures a graph cannot initialise: make the "
+                                    "object before the capture")
         self.workspace = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
         if need:
             _call(cache.index, cache.lib.seedmi_kv_attention_workspace_init, "seedmi_kv_attention_workspace_init", cache.lib,
                   self.workspace.data_ptr(), need)
-            if not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream(cache.device).synchronize()              # ready for a first call on any stream
+            torch.cuda.current_stream(cache.device).synchronize()                  # ready for a first call on any stream
         self._home = _current_stream(cache.index)
         self._ws = (self.workspace.data_ptr(), need) if need else (None, 0)
         self._fn, self._rows, self._cols = cache.lib.seedmi_kv_attention, self.slots * tokens, heads * cache.head_dim

@@ -215,7 +215,8 @@ class LlamaEngine:
         """``forward`` over caches of the caller's: input_ids int64 [B,T], slot b of ``kv`` holds ``past[b]`` positions (int32 on the device,
         at most ``past_max``; negative: idle, its logits mean nothing) and T more are appended.  ``prefix`` / ``prefix_len``: positions in
         front that all slots share, held once (``new_kv(1, n)``, filled by a call of its own).  Returns logits [B, T or 1, vocab].  The
-        caller advances ``past``; a captured call replays as it grows, up to ``past_max``."""
+        caller advances ``past``; a captured call replays as it grows, up to ``past_max``.  A call is captured after it (or a larger one) has
+        run once: a capture does not grow the engine's workspaces."""
         if input_ids.dim() != 2:
             raise ValueError("You have to specify input_ids of shape [batch, seq]")
         B, T = input_ids.shape
@@ -228,9 +229,16 @@ class LlamaEngine:
             raise ValueError(f"forward_kv: past must be {B} contiguous int32 on {self.device}")
         input_ids = input_ids.to(device=self.device, dtype=torch.int64).contiguous()
         logits = torch.empty(B * (1 if last_only else T), self.vocab_pad, dtype=self.dtype, device=self.device)
-        ws = self._workspace(B, T)
         need = self.lib.seedmi_kv_attention_workspace_bytes(kv.array, B, T, self.cfg.heads, past_max + T, prefix_len)
         with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing() and (
+                    need > (0 if self._kv_ws is None else self._kv_ws.numel()) or
+                    self.lib.seedmi_llama_workspace_bytes(C.byref(self.w), B, T) > (0 if self._ws is None else self._ws.numel())):
+                # (a capture records a workspace's initialisation and does not run it: eager calls before the first replay would start from
+                # whatever is there)
+                raise L.SeedmiError(f"forward_kv: a captured call of {B} x {T} tokens behind up to {past_max} needs larger workspaces than the "
+                                    "engine has, and a capture cannot initialise them: make the same call once before the capture")
+            ws = self._workspace(B, T)
             if need > (0 if self._kv_ws is None else self._kv_ws.numel()):
                 self._kv_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
                 L.check(self.lib.seedmi_kv_attention_workspace_init(L.ptr(self._kv_ws), need, L.stream_ptr()), "seedmi_kv_attention_workspace_init",

@@ -1,10 +1,16 @@
 """KV caches by handle, without a GPU: which host-side calls are taken, which are refused, and that a refused call leaves nothing behind."""
+import contextlib
+import ctypes as C
 import types
 
 import pytest
 import torch
 
-from seed_amd.kv_cache import KVCache
+from seed_amd import config as CFG
+from seed_amd import kv_cache
+from seed_amd import lib as L
+from seed_amd.kv_cache import KVAttention, KVCache, LayerCaches
+from seed_amd.llama_engine import LlamaEngine
 
 
 # ------------------------------------------------------------------------------------------------ rows of a call
@@ -19,3 +25,64 @@ def test_rows_that_tokens_do_not_divide_are_refused(rows, tokens):
                                                    (6, None, torch.zeros(3, dtype=torch.int32), (3, 2)), (6, 2, torch.zeros(4, dtype=torch.int32), (3, 2))])
 def test_slots_and_tokens_of_a_call(rows, tokens, lens, want):
     assert KVCache._batch(types.SimpleNamespace(slots=8 if tokens else 4), "append", rows, lens, tokens) == want
+
+
+# ------------------------------------------------------------------------------------------------ workspaces and captures
+class _Called(Exception):
+    """A stub's method that must not be reached was."""
+
+
+def _on_the_host(slots=2, heads=2, rows=4096, dim=128):
+    """A 16-bit cache whose tensors are on the CPU, for what the Python side decides by itself (no call of it may launch)."""
+    c = KVCache.__new__(KVCache)
+    c.k = c.v = torch.zeros(slots, heads, rows, dim, dtype=torch.bfloat16)
+    c.k_scale = c.v_scale = None
+    c.dtype, c.device, c.format, c.index = torch.bfloat16, torch.device("cpu"), "16", -1
+    c.slots, c.kv_heads, c.rows, c.head_dim = slots, heads, rows, dim
+    c.lib = L.load()
+    c.struct = L.KVCacheStruct(c.k.data_ptr(), c.v.data_ptr(), 0, 0, heads * rows, rows, slots, rows, heads, dim, L.KV_16BIT)
+    c._ref = C.byref(c.struct)
+    return c
+
+
+def test_an_attention_with_a_workspace_is_not_made_during_a_capture(monkeypatch):
+    """The initialisation of the arrival counters would be recorded and not run: calls before the first replay would count on whatever the
+    allocation held, and their rows stay unwritten."""
+    def reached(*a, **k):
+        raise _Called
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(kv_cache, "_call", reached)
+    cache = _on_the_host()
+    assert cache.lib.seedmi_kv_attention_workspace_bytes(cache._ref, 2, 1, 2, 0, 0) > 0
+    with pytest.raises(L.SeedmiError, match="before the capture"):
+        KVAttention(cache, heads=2)
+
+
+def _engine_on_the_host(ws, kv_ws, monkeypatch):
+    """A LlamaEngine without weights on the CPU, as forward_kv sees it up to its first library call."""
+    e = LlamaEngine.__new__(LlamaEngine)
+    e.cfg, e.dtype, e.device, e.lib = CFG.LLAMA_TINY, torch.bfloat16, torch.device("cpu"), L.load()
+    e.w = L.LlamaWeights()
+    e.w.hidden, e.w.layers, e.w.heads, e.w.ffn, e.w.vocab = e.cfg.hidden, e.cfg.layers, e.cfg.heads, e.cfg.ffn, e.cfg.vocab
+    e.vocab_pad, e.w.vocab_pad, e.w.max_pos = e.cfg.vocab, e.cfg.vocab, e.cfg.max_pos
+    e._ws, e._ws_key, e._kv_ws, e._kv_refs = ws, (0, 0), kv_ws, []
+
+    def reached(*a, **k):
+        raise _Called
+    monkeypatch.setattr(LlamaEngine, "new_workspace", reached)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    return e
+
+
+@pytest.mark.parametrize("missing", ["attention", "activations"])
+def test_forward_kv_does_not_grow_its_workspaces_during_a_capture(monkeypatch, missing):
+    """A warm-up with a smaller past_max than the captured call's: the larger workspace's counters would be initialised by the replays only."""
+    cfg = CFG.LLAMA_TINY
+    kv = LayerCaches([_on_the_host(2, cfg.heads, 4096, cfg.head_dim) for _ in range(cfg.layers)])
+    need = L.load().seedmi_kv_attention_workspace_bytes(kv.array, 2, 1, cfg.heads, 4000, 0)
+    assert need > 0
+    big = torch.zeros(1 << 24, dtype=torch.uint8)
+    e = _engine_on_the_host(big if missing == "attention" else big[:1], big[:need - 1] if missing == "attention" else big, monkeypatch)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(L.SeedmiError, match="once before the capture"):
+        e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), 3999)
