@@ -57,7 +57,7 @@ class LlamaEngine:
         self._ws = None
         self._ws_key = (0, 0)
         self._kv_ws = None                     # forward_kv's attention workspace
-        self._kv_refs = []                     # workspaces that forward_kv has used: a call captured into a graph replays on them
+        self._kv_captured = []                 # the workspaces of forward_kv calls in graphs, which replay on them
         self.past_len = 0
         self.cache_generation = 0              # bumped by resize_cache: consumers that baked cache addresses in compare it
         self._pack(state_dict)
@@ -243,8 +243,8 @@ class LlamaEngine:
                 self._kv_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
                 L.check(self.lib.seedmi_kv_attention_workspace_init(L.ptr(self._kv_ws), need, L.stream_ptr()), "seedmi_kv_attention_workspace_init",
                         self.lib)
-            if not self._kv_refs or self._kv_refs[-1][0] is not ws or self._kv_refs[-1][1] is not self._kv_ws:
-                self._kv_refs.append((ws, self._kv_ws))
+            if torch.cuda.is_current_stream_capturing() and not any(a is ws and b is self._kv_ws for a, b in self._kv_captured):
+                self._kv_captured.append((ws, self._kv_ws))
             rc = self.lib.seedmi_llama_forward_kv(C.byref(self.w), kv.array, prefix.array if prefix_len else None, prefix_len, L.ptr(input_ids), B, T,
                                                   L.ptr(past), past_max, 1 if last_only else 0, L.ptr(logits), self.vocab_pad, L.ptr(self._kv_ws),
                                                   0 if self._kv_ws is None else self._kv_ws.numel(), L.ptr(ws), ws.numel(), L.stream_ptr())

@@ -1,5 +1,7 @@
 """KV caches by handle on the GPU: calls around captures and streams, and values at the edges of the types."""
+import gc
 import math
+import weakref
 
 import pytest
 import torch
@@ -69,6 +71,35 @@ def test_forward_kv_is_captured_after_a_call_of_its_size(engine):
     with torch.cuda.graph(graph):
         out = engine.forward_kv(tok, kv, past, 240, last_only=True)
     assert torch.equal(engine.forward_kv(tok, kv, past, 240, last_only=True), want)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_forward_kv_keeps_only_the_workspaces_that_graphs_replay_on(engine):
+    """Prompts that grow step by step: every outgrown workspace is released, but for those of a captured call, whose replays go on."""
+    kv = engine.new_kv(2, 250)
+    old = []
+    for T in (3, 20, 60, 130, 200):
+        engine.forward_kv(torch.ones(1, T, dtype=torch.int64).cuda(), kv, _lens(0), 40 if T < 200 else 0, last_only=True)
+        old.append((weakref.ref(engine._ws), None if engine._kv_ws is None else weakref.ref(engine._kv_ws)))
+    gc.collect()
+    assert old[0][0]() is None and old[-1][0]() is engine._ws
+    assert len({id(w()) for w, _ in old if w() is not None}) == 1 and len({id(k()) for _, k in old if k is not None and k() is not None}) <= 1
+    small = LlamaEngine(make_llama_state_dict(CFG, seed=11, norm_jitter=0.1), CFG, device="cuda", batch_cap=4, tmax=128)
+    tok, past = torch.tensor([[5]]).cuda(), _lens(9)
+    step = lambda: small.forward_kv(tok, kv, past, 240, last_only=True)  # noqa: E731
+    want = step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = step()
+    captured = [weakref.ref(small._ws), weakref.ref(small._kv_ws)]
+    small.forward_kv(torch.ones(2, 200, dtype=torch.int64).cuda(), kv, _lens(-1, 0), 50, last_only=True)
+    small.resize_cache(tmax=64)
+    gc.collect()
+    assert all(w() is not None for w in captured) and small._ws is None
     for _ in range(3):
         graph.replay()
         torch.cuda.synchronize()

@@ -65,7 +65,7 @@ def _engine_on_the_host(ws, kv_ws, monkeypatch):
     e.w = L.LlamaWeights()
     e.w.hidden, e.w.layers, e.w.heads, e.w.ffn, e.w.vocab = e.cfg.hidden, e.cfg.layers, e.cfg.heads, e.cfg.ffn, e.cfg.vocab
     e.vocab_pad, e.w.vocab_pad, e.w.max_pos = e.cfg.vocab, e.cfg.vocab, e.cfg.max_pos
-    e._ws, e._ws_key, e._kv_ws, e._kv_refs = ws, (0, 0), kv_ws, []
+    e._ws, e._ws_key, e._kv_ws, e._kv_captured = ws, (0, 0), kv_ws, []
 
     def reached(*a, **k):
         raise _Called
