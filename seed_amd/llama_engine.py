@@ -216,7 +216,8 @@ class LlamaEngine:
         at most ``past_max``; negative: idle, its logits mean nothing) and T more are appended.  ``prefix`` / ``prefix_len``: positions in
         front that all slots share, held once (``new_kv(1, n)``, filled by a call of its own).  Returns logits [B, T or 1, vocab].  The
         caller advances ``past``; a captured call replays as it grows, up to ``past_max``.  A call is captured after it (or a larger one) has
-        run once: a capture does not grow the engine's workspaces."""
+        run once: a capture does not grow the engine's workspaces.  The engine has one set of them for all its calls: calls, and replays
+        of captured ones, run one after the other - on one stream, or with an event between two."""
         if input_ids.dim() != 2:
             raise ValueError("You have to specify input_ids of shape [batch, seq]")
         B, T = input_ids.shape
@@ -238,13 +239,22 @@ class LlamaEngine:
                 # whatever is there)
                 raise L.SeedmiError(f"forward_kv: a captured call of {B} x {T} tokens behind up to {past_max} needs larger workspaces than the "
                                     "engine has, and a capture cannot initialise them: make the same call once before the capture")
+            had = self._ws, self._kv_ws
             ws = self._workspace(B, T)
             if need > (0 if self._kv_ws is None else self._kv_ws.numel()):
                 self._kv_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
                 L.check(self.lib.seedmi_kv_attention_workspace_init(L.ptr(self._kv_ws), need, L.stream_ptr()), "seedmi_kv_attention_workspace_init",
                         self.lib)
-            if torch.cuda.is_current_stream_capturing() and not any(a is ws and b is self._kv_ws for a, b in self._kv_captured):
-                self._kv_captured.append((ws, self._kv_ws))
+            if torch.cuda.is_current_stream_capturing():
+                if not any(a is ws and b is self._kv_ws for a, b in self._kv_captured):
+                    self._kv_captured.append((ws, self._kv_ws))
+            else:
+                stream = torch.cuda.current_stream()
+                for t in (ws, self._kv_ws):
+                    if t is not None:
+                        t.record_stream(stream)                                    # (freed memory is not handed on while this stream uses it)
+                if had[0] is not ws or had[1] is not self._kv_ws:
+                    stream.synchronize()                                           # a new workspace is ready for a first call on any stream
             rc = self.lib.seedmi_llama_forward_kv(C.byref(self.w), kv.array, prefix.array if prefix_len else None, prefix_len, L.ptr(input_ids), B, T,
                                                   L.ptr(past), past_max, 1 if last_only else 0, L.ptr(logits), self.vocab_pad, L.ptr(self._kv_ws),
                                                   0 if self._kv_ws is None else self._kv_ws.numel(), L.ptr(ws), ws.numel(), L.stream_ptr())

@@ -104,3 +104,31 @@ def test_forward_kv_keeps_only_the_workspaces_that_graphs_replay_on(engine):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_new_workspaces_of_forward_kv_are_ready_for_any_stream(engine):
+    """The call that allocates them returns after their initialisation has run, on a busy stream too; calls on two streams with an event
+    between them give what one stream gives."""
+    kv, twin = engine.new_kv(2, 250), engine.new_kv(2, 250)
+    ids, tok = torch.arange(60).view(2, 30).cuda(), torch.tensor([[5], [7]]).cuda()
+    a = torch.randn(4096, 4096, device="cuda", dtype=BF)
+    b = a @ a
+    none = _lens(0, 0)
+    engine.forward_kv(tok, kv, none, 0)                                            # (the kernels are loaded; the next call's workspaces are larger)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(300):
+            torch.mm(a, a, out=b)
+        busy = torch.cuda.Event()
+        busy.record()
+        first = engine.forward_kv(ids, kv, none, 0)
+        assert busy.query()
+    torch.cuda.current_stream().wait_stream(side)
+    second = engine.forward_kv(tok, kv, _lens(30, 30), 240)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        third = engine.forward_kv(tok, kv, _lens(31, 31), 240)
+    torch.cuda.synchronize()
+    for got, x, n, most in ((first, ids, 0, 0), (second, tok, 30, 240), (third, tok, 31, 240)):
+        assert torch.equal(got, engine.forward_kv(x, twin, _lens(n, n), most))
