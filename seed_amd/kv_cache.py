@@ -127,7 +127,7 @@ class KVCache:
             if n.dtype is not torch.int32 or n.get_device() != self.index or n.numel() < batch or not n.is_contiguous():
                 raise ValueError(f"{what}: lengths must be a contiguous int32 tensor with one entry per slot on {self.device}")
             return 0, n.data_ptr()
-        return int(n), None
+        return L.int32(what, n), None
 
     def _rows_of(self, what: str, x: torch.Tensor, cols: int):
         """Row stride of x [rows, cols] in the cache's type on its device."""
@@ -156,9 +156,10 @@ class KVCache:
         rotated queries [rows, heads * head_dim].  ``qkv`` [slots * T, (heads + 2 kv_heads) * head_dim] (q | k | v), slot-major; ``cos`` /
         ``sin`` [positions, head_dim] in the cache's type; positions are ``pos_ids`` (int64 [slots * T]) or pos_base + past + t."""
         D = self.head_dim
+        heads, pos_base = L.int32("KVCache.append: heads", heads), L.int32("KVCache.append: pos_base", pos_base)
         ld = self._rows_of("KVCache.append", qkv, (heads + 2 * self.kv_heads) * D)
         B, T = self._batch("KVCache.append", qkv.shape[0], past, tokens)
-        n, lens = self._lengths("KVCache.append", past, B)
+        n, lens = self._lengths("KVCache.append: past", past, B)
         if not (cos.dtype is self.dtype and sin.dtype is self.dtype and cos.get_device() == self.index and sin.get_device() == self.index and
                 cos.dim() == 2 and cos.shape == sin.shape and cos.size(1) == D and cos.is_contiguous() and sin.is_contiguous()):
             raise ValueError(f"KVCache.append: cos / sin must be contiguous {self.dtype} [positions, {D}] on {self.device}")
@@ -182,9 +183,10 @@ class KVCache:
         """Rows start .. start + n - 1 of every slot (or of the first ``slots``) of an mx8 cache as 16-bit (keys, values), [slots, kv_heads, n,
         head_dim].  Rows that a device-resident start puts outside the cache read as zeros."""
         B = slots if slots is not None else (start.numel() if isinstance(start, torch.Tensor) else self.slots)
+        n = L.int32("KVCache.read: n", n)
         if not 1 <= B <= self.slots or n < 0:
             raise ValueError(f"KVCache.read: {n} rows of {B} of {self.slots} slots")
-        at, starts = self._lengths("KVCache.read", start, B)
+        at, starts = self._lengths("KVCache.read: start", start, B)
         shape = (B, self.kv_heads, n, self.head_dim)
         for t in (k_out, v_out):
             if t is not None and (tuple(t.shape) != shape or t.dtype is not self.dtype or t.get_device() != self.index or not t.is_contiguous()):
@@ -234,11 +236,12 @@ class KVAttention:
             raise ValueError("KVAttention: prefix and cache must have one type and one device")
         if heads < 1 or heads % cache.kv_heads or tokens < 1:
             raise ValueError(f"KVAttention: {heads} query heads on {cache.kv_heads} key heads, {tokens} tokens")
-        self.cache, self.prefix, self.prefix_len = cache, prefix, int(prefix_len)
+        heads, tokens = L.int32("KVAttention: heads", heads), L.int32("KVAttention: tokens", tokens)
+        self.cache, self.prefix, self.prefix_len = cache, prefix, L.int32("KVAttention: prefix_len", prefix_len)
         self.heads, self.tokens, self.slots = heads, tokens, cache.slots if slots is None else slots
         if not 1 <= self.slots <= cache.slots:
             raise ValueError(f"KVAttention: {self.slots} of {cache.slots} slots")
-        self.kv_max, self.causal = int(kv_max), 1 if causal else 0
+        self.kv_max, self.causal = L.int32("KVAttention: kv_max", kv_max), 1 if causal else 0
         self.scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
         self._pref = self.prefix._ref if self.prefix_len else None
         need = cache.lib.seedmi_kv_attention_workspace_bytes(cache._ref, self.slots, tokens, heads, self.kv_max, self.prefix_len)
@@ -264,8 +267,9 @@ class KVAttention:
         ldq = c._rows_of("KVAttention", q, cols)
         if q.size(0) != rows:
             raise ValueError(f"KVAttention: {q.size(0)} query rows, made for {self.slots} slots of {self.tokens}")
-        n, lens = c._lengths("KVAttention", kv_len, self.slots)
-        n += plus
+        n, lens = c._lengths("KVAttention: kv_len", kv_len, self.slots)
+        if plus:
+            n = L.int32("KVAttention: kv_len + plus", n + plus)
         if out is None:
             out, ldo = torch.empty((rows, cols), dtype=c.dtype, device=c.device), cols
         else:

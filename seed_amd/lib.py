@@ -219,6 +219,14 @@ def check(rc, what="", lib=None):
         raise SeedmiError(f"{what} failed with code {rc}: {msg}")
 
 
+def int32(what: str, n) -> int:
+    """``n`` as an argument of type int of the C ABI.  (ctypes takes the low 32 bits of a larger one without a word: 2^32 + 5 rows would be 5.)"""
+    n = int(n)
+    if not -(1 << 31) <= n < 1 << 31:
+        raise ValueError(f"{what} = {n}: beyond 32 bits")
+    return n
+
+
 def stream_ptr():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)

@@ -230,6 +230,7 @@ class LlamaEngine:
             raise ValueError(f"forward_kv: past must be {B} contiguous int32 on {self.device}")
         input_ids = input_ids.to(device=self.device, dtype=torch.int64).contiguous()
         logits = torch.empty(B * (1 if last_only else T), self.vocab_pad, dtype=self.dtype, device=self.device)
+        past_max, prefix_len = L.int32("forward_kv: past_max", past_max), L.int32("forward_kv: prefix_len", prefix_len)
         need = self.lib.seedmi_kv_attention_workspace_bytes(kv.array, B, T, self.cfg.heads, past_max + T, prefix_len)
         with torch.cuda.device(self.device):
             if torch.cuda.is_current_stream_capturing() and (

@@ -42,6 +42,7 @@ def _on_the_host(slots=2, heads=2, rows=4096, dim=128):
     c.lib = L.load()
     c.struct = L.KVCacheStruct(c.k.data_ptr(), c.v.data_ptr(), 0, 0, heads * rows, rows, slots, rows, heads, dim, L.KV_16BIT)
     c._ref = C.byref(c.struct)
+    c._append, c._read = c.lib.seedmi_kv_append, c.lib.seedmi_kv_read
     return c
 
 
@@ -86,3 +87,43 @@ def test_forward_kv_does_not_grow_its_workspaces_during_a_capture(monkeypatch, m
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(L.SeedmiError, match="once before the capture"):
         e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), 3999)
+
+
+# ------------------------------------------------------------------------------------------------ numbers beyond 32 bits
+BIG = 1 << 32
+
+
+def test_numbers_beyond_32_bits_are_refused(monkeypatch):
+    """ctypes passes the low 32 bits of an int: 2^32 + 5 rows would be 5."""
+    def reached(*a, **k):
+        raise _Called
+    monkeypatch.setattr(kv_cache, "_call", reached)
+    monkeypatch.setattr(kv_cache, "_current_stream", lambda index: 0)
+    c = _on_the_host(rows=64)
+    q, qkv = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(2, 768, dtype=torch.bfloat16)
+    cos = torch.zeros(64, 128, dtype=torch.bfloat16)
+    attn = KVAttention(c, heads=2)
+    assert attn.workspace is None
+    ok = [lambda: c.append(qkv, cos, cos, 5, heads=2), lambda: c.read(5, 2), lambda: attn(q, 5), lambda: attn(q, 5, plus=1)]
+    for call in ok:
+        with pytest.raises(_Called):
+            call()
+    bad = [lambda: c.append(qkv, cos, cos, BIG + 5, heads=2), lambda: c.append(qkv, cos, cos, 5, heads=2, pos_base=BIG), lambda: c.read(BIG, 2),
+           lambda: c.read(5, BIG), lambda: attn(q, BIG + 5), lambda: attn(q, 5, plus=BIG), lambda: attn(q, (1 << 31) - 1, plus=1),
+           lambda: KVAttention(c, heads=2, kv_max=BIG + 5), lambda: KVAttention(c, heads=2, tokens=BIG + 1),
+           lambda: KVAttention(c, heads=BIG + 2), lambda: KVAttention(c, heads=2, prefix=c, prefix_len=BIG + 1)]
+    for call in bad:
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            call()
+
+
+@pytest.mark.parametrize("kw", [dict(past_max=BIG + 5), dict(past_max=-BIG), dict(past_max=5, prefix_len=BIG + 1)])
+def test_forward_kv_refuses_numbers_beyond_32_bits(monkeypatch, kw):
+    cfg = CFG.LLAMA_TINY
+    kv = LayerCaches([_on_the_host(2, cfg.heads, 64, cfg.head_dim) for _ in range(cfg.layers)])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    e = _engine_on_the_host(None, None, monkeypatch)
+    with pytest.raises(ValueError, match="beyond 32 bits"):
+        e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), prefix=kv if "prefix_len" in kw else None, **kw)
+    with pytest.raises(_Called):
+        e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), 5)
