@@ -2026,6 +2026,10 @@ extern "C" int seedmi_llama_forward_kv(const seedmi_llama_weights_t* w, const se
         seedmi_set_error("seedmi_llama_forward_kv: null argument, bad batch / T / past_max, or prefix_len without a prefix");
         return SEEDMI_E_SHAPE;
     }
+    if (w->layers <= 0 || w->heads <= 0 || w->hidden <= 0 || w->hidden % w->heads) {
+        seedmi_set_error("seedmi_llama_forward_kv: a model of %d layers, %d heads, hidden %d", w->layers, w->heads, w->hidden);
+        return SEEDMI_E_SHAPE;
+    }
     for (int l = 0; l < w->layers; ++l) {
         if (kv[l].kv_heads != w->heads || kv[l].head_dim != w->hidden / w->heads || kv[l].slots < batch || kv[l].rows < 1) {
             seedmi_set_error("seedmi_llama_forward_kv: layer %d's cache has %d heads of %d, %d slots; the model %d heads of %d, batch %d", l,

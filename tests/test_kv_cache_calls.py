@@ -1,6 +1,9 @@
 """KV caches by handle, without a GPU: which host-side calls are taken, which are refused, and that a refused call leaves nothing behind."""
 import contextlib
 import ctypes as C
+import os
+import subprocess
+import sys
 import types
 
 import pytest
@@ -11,6 +14,8 @@ from seed_amd import kv_cache
 from seed_amd import lib as L
 from seed_amd.kv_cache import KVAttention, KVCache, LayerCaches
 from seed_amd.llama_engine import LlamaEngine
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 # ------------------------------------------------------------------------------------------------ rows of a call
@@ -127,3 +132,34 @@ def test_forward_kv_refuses_numbers_beyond_32_bits(monkeypatch, kw):
         e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), prefix=kv if "prefix_len" in kw else None, **kw)
     with pytest.raises(_Called):
         e.forward_kv(torch.zeros(2, 1, dtype=torch.int64), kv, torch.zeros(2, dtype=torch.int32), 5)
+
+
+# ------------------------------------------------------------------------------------------------ the forward at the C ABI
+FAKE = 0x10000                                            # aligned, never dereferenced on these paths
+
+
+def _handle(**kw):
+    h = L.KVCacheStruct(FAKE, FAKE, FAKE, FAKE, 2 * 64, 64, 4, 64, 2, 128, L.KV_MX8)
+    for k, v in kw.items():
+        setattr(h, k, v)
+    return h
+
+
+@pytest.mark.parametrize("model,cache", [(dict(heads=0), {}), (dict(heads=0), dict(kv_heads=0)), (dict(heads=-2), dict(kv_heads=-2)),
+                                         (dict(hidden=0), {}), (dict(hidden=255), {}), (dict(layers=0), {}), (dict(layers=-1), {})])
+def test_a_model_without_heads_or_layers_is_refused(model, cache):
+    """An error code, not a division by zero, from a process of its own."""
+    code = f"""
+import ctypes as C
+from seed_amd import lib as L
+w = L.LlamaWeights()
+for k, v in dict(dict(hidden=256, layers=1, heads=2, max_pos=64), **{model}).items():
+    setattr(w, k, v)
+h = L.KVCacheStruct({FAKE}, {FAKE}, {FAKE}, {FAKE}, 128, 64, 4, 64, 2, 128, L.KV_MX8)
+for k, v in {cache}.items():
+    setattr(h, k, v)
+kv = (L.KVCacheStruct * 1)(h)
+print(L.load().seedmi_llama_forward_kv(C.byref(w), kv, None, 0, {FAKE}, 4, 2, {FAKE}, 8, 0, {FAKE}, 64, None, 0, {FAKE}, 0, None))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and r.stdout.split()[-1] == "-1", (r.returncode, r.stderr)
