@@ -1358,9 +1358,10 @@ int check_cache(const char* who, const seedmi_kv_cache_t* c, KvView* v) {
         else { if (mx) { CALL(64, true); } else { CALL(64, false); } }  \
     } while (0)
 
-extern "C" int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv, int ldqkv, const void* pos_ids_i64, int pos_base,
-                                const void* cos_t, const void* sin_t, int max_pos, void* q_out, int ldq, int B, int T, int H, int past_len,
-                                const void* past_lens_i32, void* stream) {
+// seedmi_kv_append / seedmi_kv_attention, or their checks alone (launch == false): a path of many launches refuses before the first one
+int seedmi_kv_append_impl(const seedmi_kv_cache_t* cache, const void* qkv, int ldqkv, const void* pos_ids_i64, int pos_base, const void* cos_t,
+                          const void* sin_t, int max_pos, void* q_out, int ldq, int B, int T, int H, int past_len, const void* past_lens_i32,
+                          void* stream, bool launch) {
     KvView v;
     if (const int rc = check_cache("seedmi_kv_append", cache, &v)) return rc;
     const int hd = cache->head_dim, G = cache->kv_heads;
@@ -1391,6 +1392,7 @@ extern "C" int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv,
         seedmi_set_error("seedmi_kv_append: B * T * (H + 2 kv_heads) * head_dim / 16 = %lld: at most 2^31 - 1", total);
         return SEEDMI_E_SHAPE;
     }
+    if (!launch) return SEEDMI_OK;
 #define CALL(HD, MX)                                                                                                                         \
     hipLaunchKernelGGL((kv_append_kernel<HD, MX>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, v,              \
                        (const bf16_t*)qkv, ldqkv, (const long long*)pos_ids_i64, pos_base, (const bf16_t*)cos_t, (const bf16_t*)sin_t,       \
@@ -1398,6 +1400,13 @@ extern "C" int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv,
     KV_DISPATCH(hd, cache->format == SEEDMI_KV_MX8, CALL);
 #undef CALL
     return seedmi_check_launch("kv_append");
+}
+
+extern "C" int seedmi_kv_append(const seedmi_kv_cache_t* cache, const void* qkv, int ldqkv, const void* pos_ids_i64, int pos_base,
+                                const void* cos_t, const void* sin_t, int max_pos, void* q_out, int ldq, int B, int T, int H, int past_len,
+                                const void* past_lens_i32, void* stream) {
+    return seedmi_kv_append_impl(cache, qkv, ldqkv, pos_ids_i64, pos_base, cos_t, sin_t, max_pos, q_out, ldq, B, T, H, past_len, past_lens_i32,
+                                 stream, true);
 }
 
 extern "C" int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int B, int n, int start, const void* starts_i32,
@@ -1568,9 +1577,9 @@ static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, c
     }
 }
 
-extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq,
-                                   void* out, int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale,
-                                   int causal, void* workspace, size_t workspace_bytes, void* stream) {
+int seedmi_kv_attention_impl(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq, void* out,
+                             int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale, int causal,
+                             void* workspace, size_t workspace_bytes, void* stream, bool launch) {
     KvView own, pre;
     if (const int rc = check_cache("seedmi_kv_attention", cache, &own)) return rc;
     const int hd = cache->head_dim, G = cache->kv_heads;
@@ -1610,6 +1619,7 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
         seedmi_set_error("seedmi_kv_attention: workspace %zu bytes (need %zu, 256-byte aligned)", workspace_bytes, pl.bytes);
         return SEEDMI_E_ALIGN;
     }
+    if (!launch) return SEEDMI_OK;
     AttnArgs a = {};
     a.q = (const bf16_t*)q;
     a.out = (bf16_t*)out;
@@ -1624,4 +1634,11 @@ extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_
     KV_DISPATCH(hd, cache->format == SEEDMI_KV_MX8, CALL);
 #undef CALL
     return seedmi_check_launch("kv_attention");
+}
+
+extern "C" int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq,
+                                   void* out, int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale,
+                                   int causal, void* workspace, size_t workspace_bytes, void* stream) {
+    return seedmi_kv_attention_impl(cache, prefix, prefix_len, q, ldq, out, ldo, B, T, H, kv_len, kv_lens_i32, kv_max, scale, causal, workspace,
+                                    workspace_bytes, stream, true);
 }

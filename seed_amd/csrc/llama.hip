@@ -1907,6 +1907,17 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
     const bool fold = pk && w->norm_folded && !g_ablate_norm;
     void* const sk = (pk && t.sk && g_skinny_sk.load(std::memory_order_relaxed)) ? t.sk : nullptr;
     const bool fused_first = fold && !inputs_embeds;     // embedding rows, their fragment-major copy and the flag clear in ONE launch
+    // append and attention of layer l by cache handle; the attention's rows are row-major, so decode steps repack them for the o_proj GEMM
+    // (xn is free there: the q/k/v GEMM has consumed it, the o_proj GEMM writes it next)
+    bf16_t* const kv_rows = pk ? t.xn : t.att;
+    auto kv_step = [&](int l, bool launch) -> int {
+        CK(seedmi_kv_append_impl(&path->kv[l], t.qkv, 3 * h, nullptr, path->prefix_len, w->cos_t, w->sin_t, w->max_pos, t.q, h, batch, T, H, 0,
+                                 path->past_lens, stream, launch));
+        return seedmi_kv_attention_impl(&path->kv[l], path->prefix_len ? &path->prefix[l] : nullptr, path->prefix_len, t.q, h, kv_rows, h, batch, T,
+                                        H, T, path->past_lens, path->past_max + T, scale, 1, path->ws, path->ws_bytes, stream, launch);
+    };
+    if (path)                                            // every layer's checks before the first launch: a refused call leaves the caches alone
+        for (int l = 0; l < w->layers; ++l) CK(kv_step(l, false));
     if (inputs_embeds) {                                 // LlamaModel.forward with inputs_embeds (llama_xformer.py:543-544 skipped)
         if (hipMemcpyAsync(t.x, inputs_embeds, (size_t)M * h * 2, hipMemcpyDeviceToDevice, (hipStream_t)stream) != hipSuccess) {
             seedmi_set_error("seedmi_llama_forward_io: copying inputs_embeds failed");
@@ -1963,14 +1974,8 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
                       stream, pk, 0, sk, gsk, t.gsk_bytes));
         }
         if (path) {
-            // append and attention by cache handle; the attention's rows are row-major, so decode steps repack them for the o_proj GEMM
-            // (xn is free here: the q/k/v GEMM has consumed it, the o_proj GEMM writes it next)
-            bf16_t* const rows = pk ? t.xn : t.att;
-            CK(seedmi_kv_append(&path->kv[l], t.qkv, 3 * h, nullptr, path->prefix_len, w->cos_t, w->sin_t, w->max_pos, t.q, h, batch, T, H, 0,
-                                path->past_lens, stream));
-            CK(seedmi_kv_attention(&path->kv[l], path->prefix_len ? &path->prefix[l] : nullptr, path->prefix_len, t.q, h, rows, h, batch, T, H, T,
-                                   path->past_lens, path->past_max + T, scale, 1, path->ws, path->ws_bytes, stream));
-            if (pk) CK(seedmi_pack_activations_bf16(rows, h, t.att, M, h, stream));
+            CK(kv_step(l, true));
+            if (pk) CK(seedmi_pack_activations_bf16(kv_rows, h, t.att, M, h, stream));
         } else if (T == 1 && g_decode_fused) {
             // RoPE + cache append + attention in one launch (bit-identical to the two-kernel form below)
             CK(decode_attention_launch(t.qkv, 3 * h, past_len_dev ? nullptr : pos_i64, w->cos_t, w->sin_t, L.k_cache, L.v_cache, t.att, h,

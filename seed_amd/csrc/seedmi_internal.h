@@ -1,5 +1,6 @@
 // Internal declarations shared by the seedmi translation units (not part of the public C ABI).
 #pragma once
+#include <stddef.h>
 #include <stdint.h>
 
 // epilogue selectors of seedmi_gemm_bf16 (mirrored in include/seedmi.h and seed_amd/lib.py)
@@ -40,3 +41,12 @@ int seedmi_embed_rows_decode(const void* ids_i64, const void* table, int ldt, vo
                              int vocab, void* zero_words, int n_zero, void* stream);
 int seedmi_current_device(void);          // hipGetDevice, clamped to [0, SEEDMI_MAX_DEVICES)
 int seedmi_device_cus(int dev);           // multiProcessorCount of that device (cached)
+
+// kv_cache.hip: seedmi_kv_append / seedmi_kv_attention, or their checks alone (launch == false)
+struct seedmi_kv_cache;
+int seedmi_kv_append_impl(const seedmi_kv_cache* cache, const void* qkv, int ldqkv, const void* pos_ids_i64, int pos_base, const void* cos_t,
+                          const void* sin_t, int max_pos, void* q_out, int ldq, int B, int T, int H, int past_len, const void* past_lens_i32,
+                          void* stream, bool launch);
+int seedmi_kv_attention_impl(const seedmi_kv_cache* cache, const seedmi_kv_cache* prefix, int prefix_len, const void* q, int ldq, void* out,
+                             int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale, int causal,
+                             void* workspace, size_t workspace_bytes, void* stream, bool launch);

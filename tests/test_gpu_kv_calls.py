@@ -41,6 +41,7 @@ def test_an_attention_made_during_a_capture_is_refused():
     torch.cuda.synchronize()
     with pytest.raises(L.SeedmiError, match="before the capture"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            q + 1
             KVAttention(cache, heads=2)
     attn, graph = KVAttention(cache, heads=2), torch.cuda.CUDAGraph()
     assert attn.workspace is not None and torch.equal(attn(q, 2500), want)
@@ -63,6 +64,7 @@ def test_forward_kv_is_captured_after_a_call_of_its_size(engine):
     torch.cuda.synchronize()
     with pytest.raises(L.SeedmiError, match="once before the capture"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            tok + 1
             engine.forward_kv(tok, kv, past, 240, last_only=True)
     assert torch.equal(engine.forward_kv(tok, kv, past, 0, last_only=True), small)
     want = engine.forward_kv(tok, twin, past, 240, last_only=True)

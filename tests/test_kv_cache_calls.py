@@ -163,3 +163,39 @@ print(L.load().seedmi_llama_forward_kv(C.byref(w), kv, None, 0, {FAKE}, 4, 2, {F
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert r.returncode == 0 and r.stdout.split()[-1] == "-1", (r.returncode, r.stderr)
+
+
+def _forward_kv(kv, prefix=None, **kw):
+    w = L.LlamaWeights()
+    w.hidden, w.layers, w.heads, w.ffn, w.vocab, w.vocab_pad, w.max_pos, w.tmax, w.batch_cap = 256, 2, 2, 512, 64, 64, 4096, 64, 4
+    w.embed = w.cos_t = w.sin_t = FAKE
+    layers = (L.LlamaLayer * 2)()
+    w.layer = C.cast(layers, C.POINTER(L.LlamaLayer))
+    a = dict(plen=0, ids=FAKE, B=4, T=2, past=FAKE, past_max=8, last=0, logits=FAKE, ldl=64, aws=None, ab=0, ws=FAKE, wb=1 << 30)
+    a.update(kw)
+    kv = (L.KVCacheStruct * 2)(*kv)
+    prefix = None if prefix is None else (L.KVCacheStruct * 2)(*prefix)
+    return L.load().seedmi_llama_forward_kv(C.byref(w), kv, prefix, *a.values(), None)
+
+
+BAD_LAYERS = [(dict(format=2), -2), (dict(k=None), -1), (dict(v_scale=None), -1), (dict(v=FAKE + 8), -3), (dict(head_rows=63), -1)]
+
+
+@pytest.mark.parametrize("bad,code", BAD_LAYERS)
+def test_a_bad_cache_of_a_later_layer_is_refused_before_anything_runs(bad, code):
+    """(Here every launch fails, without a GPU: what comes back is the refusal only if nothing was launched before it.)"""
+    assert _forward_kv([_handle(), _handle(**bad)]) == code
+
+
+@pytest.mark.parametrize("bad,code", BAD_LAYERS[:4] + [(dict(rows=31), -1), (dict(head_dim=64), -1), (dict(kv_heads=1), -1),
+                                                       (dict(format=L.KV_16BIT, k_scale=None, v_scale=None), -1)])
+def test_a_bad_prefix_of_a_later_layer_is_refused_before_anything_runs(bad, code):
+    assert _forward_kv([_handle(), _handle()], [_handle(slots=1), _handle(slots=1, **bad)], plen=32, aws=FAKE, ab=1 << 20) == code
+
+
+def test_a_short_attention_workspace_is_refused_before_anything_runs():
+    kv = [_handle(rows=1 << 12, slot_rows=2 << 12, head_rows=1 << 12) for _ in range(2)]
+    need = L.load().seedmi_kv_attention_workspace_bytes(C.byref(kv[0]), 1, 1, 2, 4001, 0)
+    assert need > 0
+    for ws, n in ((None, 0), (FAKE, need - 1), (FAKE + 128, need)):
+        assert _forward_kv(kv, B=1, T=1, past_max=4000, aws=ws, ab=n) == -3
