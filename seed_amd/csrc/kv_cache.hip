@@ -254,6 +254,18 @@ SEEDMI_DEVINL float rows_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 SEEDMI_DEVINL float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+// acc + lo + hi of a word of two 16-bit elements: a dot product with ones
+SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
+#ifdef SEEDMI_F16
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(hw_f16x2, w), __builtin_bit_cast(hw_f16x2, 0x3c003c00u), acc, false);
+#else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, w), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), acc, false);
+#endif
+}
+// The sum of a row is that of its probabilities as they are rounded for the product with the values: out is then a mean of the values with
+// weights that add up to one, in every kernel.  (A sum of unrounded ones is off by what the roundings have in common: 387 equal scores of 400
+// made every output 0.92 half steps of the type too small.)
+SEEDMI_DEVINL float add_probabilities(const uint4& w, float acc) { return add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, acc)))); }
 
 // not finite: exponent field all ones, in both halves of a word of 16-bit elements
 SEEDMI_DEVINL uint32_t exp_mask16() {
@@ -615,11 +627,10 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
-                    l[u] += e[kt][r];
-                }
-            pf[u] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0][0], e[0][1]), pack2bf(e[0][2], e[0][3]), pack2bf(e[1][0], e[1][1]), pack2bf(e[1][2], e[1][3])));
+                for (int r = 0; r < 4; ++r) e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
+            const uint4 w = make_uint4(pack2bf(e[0][0], e[0][1]), pack2bf(e[0][2], e[0][3]), pack2bf(e[1][0], e[1][1]), pack2bf(e[1][2], e[1][3]));
+            l[u] = add_probabilities(w, l[u]);
+            pf[u] = __builtin_bit_cast(bf16x8, w);
         }
         if (mixed) {
             // Values that are not finite in a tile that some rows do not see whole: 0 * inf must not reach a row that does not see the key.
@@ -890,11 +901,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
                 for (int kk = 0; kk < 2; ++kk) {
                     float e[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
-                        l[u] += e[j];
-                    }
-                    pf[u][kk] = __builtin_bit_cast(bf16x8, make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7])));
+                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                    const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
+                    l[u] = add_probabilities(w, l[u]);
+                    pf[u][kk] = __builtin_bit_cast(bf16x8, w);
                 }
             }
         }
@@ -978,14 +988,6 @@ SEEDMI_DEVINL f32x16 mfma_32x32x16(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(hw_f16x8, a), __builtin_bit_cast(hw_f16x8, b), c, 0, 0, 0);
 #else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-#endif
-}
-// acc + lo + hi of a word of two 16-bit elements: a dot product with ones
-SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
-#ifdef SEEDMI_F16
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(hw_f16x2, w), __builtin_bit_cast(hw_f16x2, 0x3c003c00u), acc, false);
-#else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, w), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), acc, false);
 #endif
 }
 template <int HD>
@@ -1201,7 +1203,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 #pragma unroll
             for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], a.c2, -ref));
             const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
-            l = add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, l))));           // (the rounded ones, as the product takes them)
+            l = add_probabilities(w, l);
             pf[ks] = __builtin_bit_cast(bf16x8, w);
         }
     };

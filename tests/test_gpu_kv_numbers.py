@@ -1,0 +1,57 @@
+"""Attention over KV caches on the GPU where its numbers are at their edges.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
+import math
+
+import pytest
+import torch
+
+from seed_amd.kv_cache import KVAttention, KVCache
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+ROWS = [1, 20, 60, 100, 300]                                                       # query rows: a case for each block size
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _cache(k, v, dtype, rows=None):
+    """k, v [heads, n, D] -> a 16-bit cache of one slot, rows behind the n poisoned."""
+    G, n, D = k.shape
+    kc, vc = (torch.full((1, G, rows or n, D), float("nan"), dtype=dtype).cuda() for _ in range(2))
+    kc[0, :, :n], vc[0, :, :n] = k.to(dtype).cuda(), v.to(dtype).cuda()
+    return KVCache.wrap(kc, vc)
+
+
+def _biased_score(dtype):
+    """A score whose probability exp(score) loses nearly half a step when it is rounded."""
+    s = -(torch.arange(1, 1024, dtype=torch.float64) / 512).to(dtype).double()
+    p = torch.exp(s)
+    return s[torch.argmax((p - p.to(dtype).double()) / p)].item()
+
+
+# ------------------------------------------------------------------------------------------------ normalisation
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T", ROWS)
+def test_weights_add_up_to_one_after_rounding(dtype, T):
+    """400 keys, the first of every 32 ahead of the others, whose common probability is rounded down by nearly half a step h: divided by a sum
+    of unrounded probabilities every output would be too small by about that.  N outputs are means of values in 1 .. 2; their own
+    roundings are off by at most h each and independent, so that the mean of N of them stays within 6 standard deviations, 6 h / sqrt(3 N);
+    the keys ahead have a weight below 0.12 together, off by h: 0.12 h.  fp32 sums of 400 terms: 800 * 2^-24."""
+    n, D, h = 400, 128, _half(dtype)
+    s = _biased_score(dtype)
+    k = torch.full((2, n, D), 0.0)
+    k[:, :, 0] = s
+    k[:, ::32, 0] = 0.0
+    v = (1 + torch.rand(2, n, D, generator=torch.Generator().manual_seed(4))).to(dtype)
+    q = torch.zeros(T, 2, D)
+    q[:, :, 0] = 1.0
+    out = KVAttention(_cache(k, v, dtype), heads=2, tokens=T, scale=1.0, causal=False)(q.view(T, 2 * D).to(dtype).cuda(), n)
+    w = torch.softmax(k[:, :, 0].double(), -1)
+    assert w[0, ::32].sum() < 0.12
+    want = (w.unsqueeze(-1) * v.double()).sum(1)
+    got = out.cpu().double().view(T, 2, D)
+    assert torch.equal(got, got[:1].expand_as(got))                                # equal queries
+    mean = ((got[0] - want) / want).mean().item()
+    assert abs(mean) <= h * (6 / math.sqrt(3 * 2 * D) + 0.12) + 800 * 2.0 ** -24, (mean / h)
