@@ -188,8 +188,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, bf16_t* __
 // Query rows that read the same keys form a GROUP: the T * (H / G) rows of a (slot, key head) over the slot's own rows, or all
 // B * T * (H / G) rows of a key head over the shared prefix.  Row r of a group is token row base + r / GH (GH = H / G), head g * GH + r % GH.
 //
-// With s_j = c q.k_j (c = scale * log2 e) a range of keys gives m = max s_j, l = sum 2^(s_j - m), o = sum 2^(s_j - m) v_j; ranges join by
-// M = max m, (l, o) = sum 2^(m - M) (l, o), and out = o / l.
+// With s_j = c q.k_j (c = scale * log2 e) a range of keys gives m = reference(max s_j), l = sum 2^(s_j - m), o = sum 2^(s_j - m) v_j; ranges
+// join by M = max m, (l, o) = sum 2^(m - M) (l, o), and out = o / l.
 struct AttnPass {                                       // one pass: the slots' own rows, or the shared prefix
     KvView c;                                            // the slots' cache, or the prefix as a cache of one slot
     const int* kv_lens;
@@ -266,6 +266,17 @@ SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
 // weights that add up to one, in every kernel.  (A sum of unrounded ones is off by what the roundings have in common: 387 equal scores of 400
 // made every output 0.92 half steps of the type too small.)
 SEEDMI_DEVINL float add_probabilities(const uint4& w, float acc) { return add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, acc)))); }
+
+// What a row's exponents are taken against, given its largest score so far (in base-2 exponents): a probability leaves as 2^(score - reference),
+// rounded to the element.  bf16: the largest score, probabilities <= 1.  fp16 ends at 2^-25, far above what many thousand keys may add up from:
+// 15 less, so that probabilities reach from 2^15 down to 2^-25, 2^-40 of the largest.  Sums and values have the factor in common.
+SEEDMI_DEVINL float reference(float m) {
+#ifdef SEEDMI_F16
+    return m == -INFINITY ? 0.f : m - 15.f;
+#else
+    return m == -INFINITY ? 0.f : m;
+#endif
+}
 
 // not finite: exponent field all ones, in both halves of a word of 16-bit elements
 SEEDMI_DEVINL uint32_t exp_mask16() {
@@ -544,7 +555,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 
     bf16x8 qf[MT][KS];
     int seen[MT];
-    float m[MT], l[MT];
+    float m[MT], ref[MT], l[MT];                         // largest score, reference(), sum
     f32x4 o[MT][NT];
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
@@ -560,7 +571,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
             qf[u][ks] = __builtin_bit_cast(bf16x8, v);
         }
         m[u] = -INFINITY;
-        l[u] = 0.f;
+        ref[u] = l[u] = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -612,22 +623,22 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
             }
             float tm = max3(max3(s[u][0][0], s[u][0][1], s[u][0][2]), max3(s[u][0][3], s[u][1][0], s[u][1][1]), max2(s[u][1][2], s[u][1][3]));
             tm = rows_max(tm) * a.c2;
-            const float mn = fmaxf(m[u], tm);
-            if (__any(mn > m[u])) {                      // a new maximum: what is summed so far is scaled down
-                const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
+            if (__any(tm > m[u])) {                      // a new maximum (a NaN is none): what is summed so far is scaled down
+                const float mn = fmaxf(m[u], tm), rn = reference(mn);
+                const float f = m[u] == -INFINITY ? 0.f : exp2_hw(ref[u] - rn);
                 l[u] *= f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
                 m[u] = mn;
+                ref[u] = rn;
             }
-            const float ref = mn == -INFINITY ? 0.f : mn;
             float e[2][4];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref));
+                for (int r = 0; r < 4; ++r) e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref[u]));
             const uint4 w = make_uint4(pack2bf(e[0][0], e[0][1]), pack2bf(e[0][2], e[0][3]), pack2bf(e[1][0], e[1][1]), pack2bf(e[1][2], e[1][3]));
             l[u] = add_probabilities(w, l[u]);
             pf[u] = __builtin_bit_cast(bf16x8, w);
@@ -671,14 +682,14 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     float* so = (float*)sm;
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
-        const float lsum = rows_sum(l[u]);
+        const float lsum = rows_sum(l[u]), mr = m[u] == -INFINITY ? LOWEST : ref[u];
         __syncthreads();
-        if (g4 == 0) sml[wave][li] = make_float2(m[u], lsum);
+        if (g4 == 0) sml[wave][li] = make_float2(mr, lsum);
         __syncthreads();
         float M = LOWEST;                                // (finite: a sum that is NaN stays NaN, one that is 0 is left out)
 #pragma unroll
         for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w][li].x);
-        const float f = exp2_hw(fmaxf(m[u], LOWEST) - M);
+        const float f = exp2_hw(mr - M);
         // channel quads 4 (4 n + g) of row li, XOR-ed with the row
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -694,7 +705,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 #pragma unroll
         for (int w = 0; w < 4; ++w) Mr = fmaxf(Mr, sml[w][row].x);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) L += sml[w][row].y * exp2_hw(fmaxf(sml[w][row].x, LOWEST) - Mr);
+        for (int w = 0; w < 4; ++w) L += sml[w][row].y * exp2_hw(sml[w][row].x - Mr);
         if (r < r_end) {
             constexpr int Q = HD / 64;                   // quads of a thread
             const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
@@ -813,7 +824,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 
     bf16x8 qf[MT][KS];
     int seen[MT];
-    float m[MT], l[MT];
+    float m[MT], ref[MT], l[MT];                         // largest score, reference(), sum
     f32x4 o[MT][NT];
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
@@ -828,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
             qf[u][ks] = __builtin_bit_cast(bf16x8, v);
         }
         m[u] = -INFINITY;
-        l[u] = 0.f;
+        ref[u] = l[u] = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -886,22 +897,22 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt) tm = max3(max3(tm, s[u][kt][0], s[u][kt][1]), s[u][kt][2], s[u][kt][3]);
                 tm = rows_max(tm) * a.c2;
-                const float mn = fmaxf(m[u], tm);
-                if (__any(mn > m[u])) {
-                    const float f = mn == -INFINITY ? 1.f : exp2_hw(m[u] - mn);
+                if (__any(tm > m[u])) {
+                    const float mn = fmaxf(m[u], tm), rn = reference(mn);
+                    const float f = m[u] == -INFINITY ? 0.f : exp2_hw(ref[u] - rn);
                     l[u] *= f;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
                     m[u] = mn;
+                    ref[u] = rn;
                 }
-                const float ref = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
                     float e[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref));
+                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref[u]));
                     const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
                     l[u] = add_probabilities(w, l[u]);
                     pf[u][kk] = __builtin_bit_cast(bf16x8, w);
@@ -961,7 +972,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 #pragma unroll
                 for (int n = 0; n < NT; ++n) *(f32x4*)(a.o_part + at * HD + 16 * n + 4 * g4) = o[u][n];
             }
-            if (g4 == 0) a.ml_part[at] = make_float2(fmaxf(m[u], LOWEST), L);
+            if (g4 == 0) a.ml_part[at] = make_float2(m[u] == -INFINITY ? LOWEST : ref[u], L);
         }
     }
 }
@@ -1110,7 +1121,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
             qf[0][ks] = __builtin_bit_cast(bf16x8, v);
         }
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, ref = 0.f, l = 0.f;             // largest score, reference(), sum
     f32x16 o[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -1186,17 +1197,17 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         for (int d = 1; d < 16; ++d) tm = max3(tm, s[0][d], s[1][d]);
         auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
         tm = max2(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c2;
-        const float mn = fmaxf(m, tm);                   // (a NaN among the scores is in the sums, whatever the maximum)
-        if (__any(mn > m)) {
-            const float f = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
+        if (__any(tm > m)) {                             // (a NaN among the scores is in the sums, whatever the maximum)
+            const float mn = fmaxf(m, tm), rn = reference(mn);
+            const float f = m == -INFINITY ? 0.f : exp2_hw(ref - rn);
             l *= f;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int d = 0; d < 16; ++d) o[i][d] *= f;
             m = mn;
+            ref = rn;
         }
-        const float ref = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             float e[8];
@@ -1281,7 +1292,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 for (int e = 0; e < 4; ++e)
                     *(f32x4*)(a.o_part + at * HD + 32 * i + 8 * e + 4 * h) = (f32x4){o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
         }
-        if (h == 0) a.ml_part[at] = make_float2(fmaxf(m, LOWEST), L);
+        if (h == 0) a.ml_part[at] = make_float2(m == -INFINITY ? LOWEST : ref, L);
     }
 }
 

@@ -1,4 +1,5 @@
-"""Attention over KV caches on the GPU where its numbers are at their edges.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
+"""Attention over KV caches on the GPU where its numbers are at their edges: how the weights are normalised, tails of small weights.  Every
+kernel: 1 - 32, 33 - 128 and more query rows per key head."""
 import math
 
 import pytest
@@ -55,3 +56,48 @@ def test_weights_add_up_to_one_after_rounding(dtype, T):
     assert torch.equal(got, got[:1].expand_as(got))                                # equal queries
     mean = ((got[0] - want) / want).mean().item()
     assert abs(mean) <= h * (6 / math.sqrt(3 * 2 * D) + 0.12) + 800 * 2.0 ** -24, (mean / h)
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("T", ROWS)
+def test_a_long_tail_of_small_weights_in_fp16(T, prefix):
+    """One key ahead of 60000 whose probabilities are 2^-26.2 of its own, below fp16's smallest subnormal number: together they are 7.8e-4 of
+    the sum and, the first value being 0, all of the output.  Roundings: output and probabilities h each, fp32 sums of n terms (2 n 2^-24),
+    exponent 1e-5."""
+    n, D, h = 60001, 64, _half(HF)
+    s = -18.1875
+    k, v = torch.zeros(1, n, D), torch.ones(1, n, D)
+    k[:, 1:, 0] = s
+    v[:, 0] = 0.0
+    q = torch.zeros(T, D)
+    q[:, 0] = 1.0
+    q = q.to(HF).cuda()
+    if prefix:                                                                     # the tail shared, the key ahead the slot's own
+        tail = _cache(k[:, 1:], v[:, 1:], HF)
+        cache = _cache(k[:, :1], v[:, :1], HF)
+        out = KVAttention(cache, heads=1, tokens=T, scale=1.0, causal=False, prefix=tail, prefix_len=n - 1)(q, 1)
+    else:
+        out = KVAttention(_cache(k, v, HF), heads=1, tokens=T, scale=1.0, causal=False)(q, n)
+    share = (n - 1) * math.exp(s)
+    want = share / (1 + share)
+    off = (out.double() - want).abs().max().item()
+    assert off <= want * (2.1 * h + 2 * n * 2.0 ** -24 + 1e-5), (off / want)
+
+
+@pytest.mark.parametrize("T", ROWS)
+def test_small_weights_beside_large_ones_in_fp16(T):
+    """The first of every 32 keys ahead of the 31 others, whose probabilities of 2^-26.2 and values of 60000 make the output: it must not
+    depend on which keys a workgroup takes together.  Roundings as above."""
+    n, D, h = 2080, 64, _half(HF)
+    s = -18.1875
+    k, v = torch.zeros(1, n, D), torch.full((1, n, D), 60000.0).to(HF)
+    k[:, :, 0] = s
+    k[:, ::32, 0] = 0.0
+    v[:, ::32] = 0.0
+    q = torch.zeros(T, D)
+    q[:, 0] = 1.0
+    out = KVAttention(_cache(k, v, HF), heads=1, tokens=T, scale=1.0, causal=False)(q.to(HF).cuda(), n)
+    share = 31 * math.exp(s)
+    want = v[0, 1, 0].item() * share / (1 + share)
+    off = (out.double() - want).abs().max().item()
+    assert off <= want * (2.1 * h + 2 * n * 2.0 ** -24 + 1e-5), (off / want)
