@@ -267,12 +267,21 @@ SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
 // made every output 0.92 half steps of the type too small.)
 SEEDMI_DEVINL float add_probabilities(const uint4& w, float acc) { return add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, acc)))); }
 
+// a product that is rounded before it is used (the compiler would be free to fuse it)
+SEEDMI_DEVINL float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
 // What a row's exponents are taken against, given its largest score so far (in base-2 exponents): a probability leaves as 2^(score - reference),
 // rounded to the element.  bf16: the largest score, probabilities <= 1.  fp16 ends at 2^-25, far above what many thousand keys may add up from:
 // 15 less, so that probabilities reach from 2^15 down to 2^-25, 2^-40 of the largest.  Sums and values have the factor in common.
+// FAR: from there on score and reference are rounded by more than a sixteenth before they are subtracted, and the fused s c - reference of the
+// largest score, the rounding of s c, would no longer be near zero (2^32 and more: a probability of 2^128 or of 0).  A wave with a reference
+// beyond it rounds s c like the reference, so that the largest score's exponent is exactly 0, and takes no 15 off.
+constexpr float FAR = 0x1p20f;
 SEEDMI_DEVINL float reference(float m) {
 #ifdef SEEDMI_F16
-    return m == -INFINITY ? 0.f : m - 15.f;
+    return m == -INFINITY ? 0.f : fabsf(m) < FAR ? m - 15.f : m;
 #else
     return m == -INFINITY ? 0.f : m;
 #endif
@@ -576,6 +585,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     char* lds = sm + wave * VBYTES;
+    bool far = false;                                    // (wave-uniform) a reference beyond FAR
 
     arrived(qf);
 #pragma unroll 1
@@ -633,12 +643,20 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
                     for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
                 m[u] = mn;
                 ref[u] = rn;
+                far |= __any(fabsf(rn) >= FAR);
             }
+            if (far) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[u][kt][r] = rounded(s[u][kt][r] * a.c2);
+            }
+            const float mul = far ? 1.f : a.c2;
             float e[2][4];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) e[kt][r] = exp2_hw(fmaf(s[u][kt][r], a.c2, -ref[u]));
+                for (int r = 0; r < 4; ++r) e[kt][r] = exp2_hw(fmaf(s[u][kt][r], mul, -ref[u]));
             const uint4 w = make_uint4(pack2bf(e[0][0], e[0][1]), pack2bf(e[0][2], e[0][3]), pack2bf(e[1][0], e[1][1]), pack2bf(e[1][2], e[1][3]));
             l[u] = add_probabilities(w, l[u]);
             pf[u] = __builtin_bit_cast(bf16x8, w);
@@ -843,6 +861,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[u][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    bool far = false;                                    // (wave-uniform) a reference beyond FAR
     arrived(qf);
     if (t_begin < t_end) {
         stage_store(st, sm, sm + 2 * KB, tid);
@@ -907,12 +926,20 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
                         for (int r = 0; r < 4; ++r) o[u][n][r] *= f;
                     m[u] = mn;
                     ref[u] = rn;
+                    far |= __any(fabsf(rn) >= FAR);
                 }
+                if (far) {
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[u][kt][r] = rounded(s[u][kt][r] * a.c2);
+                }
+                const float mul = far ? 1.f : a.c2;
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
                     float e[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], a.c2, -ref[u]));
+                    for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[u][2 * kk + (j >> 2)][j & 3], mul, -ref[u]));
                     const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
                     l[u] = add_probabilities(w, l[u]);
                     pf[u][kk] = __builtin_bit_cast(bf16x8, w);
@@ -1122,6 +1149,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         }
     }
     float m = -INFINITY, ref = 0.f, l = 0.f;             // largest score, reference(), sum
+    bool far = false;                                    // (wave-uniform) a reference beyond FAR
     f32x16 o[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -1207,12 +1235,20 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 for (int d = 0; d < 16; ++d) o[i][d] *= f;
             m = mn;
             ref = rn;
+            far |= __any(fabsf(rn) >= FAR);
         }
+        if (far) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int d = 0; d < 16; ++d) s[kt][d] = rounded(s[kt][d] * a.c2);
+        }
+        const float mul = far ? 1.f : a.c2;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             float e[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], a.c2, -ref));
+            for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], mul, -ref));
             const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
             l = add_probabilities(w, l);
             pf[ks] = __builtin_bit_cast(bf16x8, w);

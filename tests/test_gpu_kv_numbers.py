@@ -1,5 +1,5 @@
-"""Attention over KV caches on the GPU where its numbers are at their edges: how the weights are normalised, tails of small weights.  Every
-kernel: 1 - 32, 33 - 128 and more query rows per key head."""
+"""Attention over KV caches on the GPU where its numbers are at their edges: how the weights are normalised, tails of small weights, scores far
+beyond those of a trained model.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
 import math
 
 import pytest
@@ -101,3 +101,44 @@ def test_small_weights_beside_large_ones_in_fp16(T):
     want = v[0, 1, 0].item() * share / (1 + share)
     off = (out.double() - want).abs().max().item()
     assert off <= want * (2.1 * h + 2 * n * 2.0 ** -24 + 1e-5), (off / want)
+
+
+# ------------------------------------------------------------------------------------------------ scores far from zero
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("magnitude", [2.0 ** 11, 2.0 ** 13, 2.0 ** 15])
+@pytest.mark.parametrize("T", ROWS)
+def test_scores_of_billions(dtype, sign, magnitude, T):
+    """q k of 2^29 to 2^37 in exact steps, times 0.127: one key ahead by a sixteenth takes all and its value comes out exactly (weights 1 and 0);
+    two keys ahead share: off by the rounding of the mean."""
+    n, D = 330, 128
+    for ahead in ((7,), (7, 11)):
+        k = torch.full((1, n, D), sign * magnitude)
+        for j in ahead:
+            k[0, j] *= 1 + sign / 16
+        v = torch.randn(1, n, D, generator=torch.Generator().manual_seed(5)).to(dtype)
+        q = torch.full((T, D), magnitude).to(dtype).cuda()
+        out = KVAttention(_cache(k, v, dtype), heads=1, tokens=T, scale=0.127)(q, n).cpu().double()
+        want = v[0, list(ahead)].double().mean(0)
+        off = (out - want).abs()
+        assert (off <= (0 if len(ahead) == 1 else 1) * _half(dtype) * want.abs() * 1.01 + (0 if len(ahead) == 1 else 2.0 ** -25)).all(), (ahead, off.max().item())
+
+
+@pytest.mark.parametrize("T", ROWS)
+def test_scores_of_billions_behind_a_prefix_and_over_split_keys(T):
+    """The same where parts of the keys are joined: the key ahead in the prefix, in the own rows, and in both."""
+    D, P, n, m = 128, 1500, 330, 2.0 ** 15
+    v, pv = (torch.randn(1, r, D, generator=torch.Generator().manual_seed(r)).to(BF) for r in (n, P))
+    q = torch.full((T, D), m).to(BF).cuda()
+    for own, shared in ((3, None), (None, 900), (3, 900)):
+        k, pk = torch.full((1, n, D), -m), torch.full((1, P, D), -m)
+        rows = []
+        if own is not None:
+            k[0, own] *= 0.75
+            rows.append(v[0, own])
+        if shared is not None:
+            pk[0, shared] *= 0.75
+            rows.append(pv[0, shared])
+        out = KVAttention(_cache(k, v, BF), heads=1, tokens=T, scale=0.127, prefix=_cache(pk, pv, BF), prefix_len=P)(q, n).cpu().double()
+        want = torch.stack(rows).double().mean(0)
+        assert ((out - want).abs() <= (len(rows) - 1) * _half(BF) * 1.01 * want.abs()).all()
