@@ -1148,8 +1148,9 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
             qf[0][ks] = __builtin_bit_cast(bf16x8, v);
         }
     }
-    float m = -INFINITY, ref = 0.f, l = 0.f;             // largest score, reference(), sum
-    bool far = false;                                    // (wave-uniform) a reference beyond FAR
+    float m = -INFINITY, nref = 0.f, l = 0.f;            // largest score, -reference() (as the exponents take it), sum
+    unsigned long long far = 0;                          // rows with a reference beyond FAR: their wave always takes the branch of a new
+    float mul = a.c2;                                    // maximum, the others have no second one (it costs 4 us of 192)
     f32x16 o[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -1225,30 +1226,30 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
         for (int d = 1; d < 16; ++d) tm = max3(tm, s[0][d], s[1][d]);
         auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
         tm = max2(__uint_as_float(w[0]), __uint_as_float(w[1])) * a.c2;
-        if (__any(tm > m)) {                             // (a NaN among the scores is in the sums, whatever the maximum)
+        if ((__ballot(tm > m) | far) != 0) {             // (a NaN among the scores is in the sums, whatever the maximum)
             const float mn = fmaxf(m, tm), rn = reference(mn);
-            const float f = m == -INFINITY ? 0.f : exp2_hw(ref - rn);
+            const float f = m == -INFINITY ? 0.f : exp2_hw(-nref - rn);
             l *= f;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int d = 0; d < 16; ++d) o[i][d] *= f;
             m = mn;
-            ref = rn;
-            far |= __any(fabsf(rn) >= FAR);
-        }
-        if (far) {
+            nref = -rn;
+            far |= __ballot(fabsf(rn) >= FAR);
+            if (far) {
+                mul = 1.f;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+                for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int d = 0; d < 16; ++d) s[kt][d] = rounded(s[kt][d] * a.c2);
+                    for (int d = 0; d < 16; ++d) s[kt][d] = rounded(s[kt][d] * a.c2);
+            }
         }
-        const float mul = far ? 1.f : a.c2;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             float e[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], mul, -ref));
+            for (int j = 0; j < 8; ++j) e[j] = exp2_hw(fmaf(s[ks >> 1][8 * (ks & 1) + j], mul, nref));
             const uint4 w = make_uint4(pack2bf(e[0], e[1]), pack2bf(e[2], e[3]), pack2bf(e[4], e[5]), pack2bf(e[6], e[7]));
             l = add_probabilities(w, l);
             pf[ks] = __builtin_bit_cast(bf16x8, w);
@@ -1328,7 +1329,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
                 for (int e = 0; e < 4; ++e)
                     *(f32x4*)(a.o_part + at * HD + 32 * i + 8 * e + 4 * h) = (f32x4){o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
         }
-        if (h == 0) a.ml_part[at] = make_float2(m == -INFINITY ? LOWEST : ref, L);
+        if (h == 0) a.ml_part[at] = make_float2(m == -INFINITY ? LOWEST : -nref, L);
     }
 }
 
