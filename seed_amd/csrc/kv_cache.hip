@@ -224,13 +224,16 @@ SEEDMI_DEVINL AttnPass pass_of(const AttnArgs& a, unsigned& block) {
 }
 
 // rows of a pass's slot that count: kv_len, on top of what the slot's own length says where there is one (negative: an idle slot), within the cache
-SEEDMI_DEVINL int rows_held(const AttnPass& p, int slot) {
-    int n = p.kv_len;
-    if (p.kv_lens && !p.shared) {
-        const int own = p.kv_lens[slot];
-        n = own < 0 ? 0 : min(own, p.c.rows) + n;
+SEEDMI_DEVINL int rows_of_slot(const int* kv_lens, int kv_len, int rows, int slot) {
+    int n = kv_len;
+    if (kv_lens) {
+        const int own = kv_lens[slot];
+        n = own < 0 ? 0 : min(own, rows) + n;
     }
-    return __builtin_amdgcn_readfirstlane(max(0, min(n, p.c.rows)));
+    return max(0, min(n, rows));
+}
+SEEDMI_DEVINL int rows_held(const AttnPass& p, int slot) {
+    return __builtin_amdgcn_readfirstlane(rows_of_slot(p.shared ? nullptr : p.kv_lens, p.kv_len, p.c.rows, slot));
 }
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -436,8 +439,11 @@ SEEDMI_DEVINL void join_part(float& M, float& L, f32x4& o, float m, float l, con
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + v[i] * f1;
 }
-SEEDMI_DEVINL void store_row_quad(bf16_t* dst, float L, const f32x4& o) {
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+// 1 / the sum of a row.  A row that sees no key gives zeros; one that sees keys and has no weights, its scores all -infinity, the formula's
+// 0 / 0, NaN.
+SEEDMI_DEVINL float inverse_sum(float L, bool sees) { return L != 0.f ? 1.f / L : sees ? __uint_as_float(0x7fc00000u) : 0.f; }
+SEEDMI_DEVINL void store_row_quad(bf16_t* dst, float L, bool sees, const f32x4& o) {
+    const float inv = inverse_sum(L, sees);
     *(uint2*)dst = make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
 }
 // Parts that another workgroup of the same launch will read, maybe on another XCD with an L2 of its own: device-scope accesses, which go past
@@ -463,10 +469,10 @@ SEEDMI_DEVINL float2 load_pair(const float* p) {
     return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
 }
 // The last workgroup of a unit to get here joins the unit's rows, in the order of their parts whoever is last: no second launch.  Rows
-// first .. + n of the group that starts at token `base`, key head kvh.  Every part's stores are past the L2s (waited for) before the
+// first .. + n of the group that starts at token `base`, key head kvh; token row t of the group sees seen0 + t * seen_step keys (or none).  Every part's stores are past the L2s (waited for) before the
 // workgroup's arrival is counted; the counter wraps to zero with the last arrival.  Workgroups wait for nobody.
 template <int HD>
-SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh, int first, int n, float* lds) {
+SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh, int first, int n, int seen0, int seen_step, float* lds) {
     constexpr int LPR = HD / 4, SLOTS = 256 / LPR, BATCH = 4;
     __shared__ unsigned s_last;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's stores have reached memory ...
@@ -511,7 +517,7 @@ SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh,
             if (w == 0)
                 for (int k = 1; k < jw; ++k) join_part(M, L, o, sl[slot + k].x, sl[slot + k].y, so[threadIdx.x + k * LPR]);
         }
-        if (on && w == 0) store_row_quad(a.out + (size_t)token * a.ldo + head * HD + 4 * c, L, o);
+        if (on && w == 0) store_row_quad(a.out + (size_t)token * a.ldo + head * HD + 4 * c, L, seen0 + r / a.GH * seen_step > 0, o);
     }
 }
 
@@ -738,7 +744,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
                     for (int d = 0; d < 4; ++d) v[d] += x[d];
                 }
                 if (a.parts == 1) {
-                    const float inv = L == 0.f ? 0.f : 1.f / L;
+                    const float inv = inverse_sum(L, (causal ? len - a.T + r / a.GH + 1 : len) > 0);
                     *(uint2*)(a.out + (size_t)token * a.ldo + head * HD + 4 * quad) = make_uint2(pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv));
                 } else {
                     const long long at = (long long)(p.part0 + split) * a.rows + (long long)token * a.H + head;
@@ -751,7 +757,9 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
     if (a.arrivals) {
         const int unit = a.unit_rows ? kvh : group * p.row_blocks + rb;
         const int first = a.unit_rows ? 0 : r0, n_rows = a.unit_rows ? a.unit_rows : r_end - r0;
-        join_in_place<HD>(a, unit, a.unit_rows ? 0 : base, kvh, first, n_rows, (float*)sm);
+        // (a unit of two passes: every row sees the prefix)
+        join_in_place<HD>(a, unit, a.unit_rows ? 0 : base, kvh, first, n_rows, a.unit_rows ? 1 : causal ? len - a.T + 1 : len,
+                          a.unit_rows ? 0 : causal, (float*)sm);
     }
 }
 
@@ -988,7 +996,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
         if (r >= r_end) continue;
         const int token = base + r / a.GH, head = kvh * a.GH + r % a.GH;
         if (a.parts == 1) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
+            const float inv = inverse_sum(L, seen[u] > 0);
             bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * g4;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -1313,7 +1321,7 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
     const float L = __uint_as_float(w[0]) + __uint_as_float(w[1]);
     if (!on) return;
     if (a.parts == 1) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = inverse_sum(L, seen > 0);
         bf16_t* op = a.out + (size_t)token * a.ldo + head * HD + 4 * h;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -1336,9 +1344,10 @@ __global__ __launch_bounds__(512) void kv_attention_phased_kernel(const AttnArgs
 // The parts of every row joined.  Thread = 4 channels of a row and every JW-th of its parts (few rows have many parts: a thread that walked
 // them all would wait for one memory round trip after the other); the JW partial sums meet in the LDS.  JW = 8 from five parts on (48 slots
 // behind a prefix, 33 parts: 61 us in all against 72 with 1), 1 below (64 K rows of two parts: 110 us in all against 136 with 8).
+struct JoinSees { const int* kv_lens; int kv_len, rows, T, causal, prefix; };              // what rows_of_slot takes; with a prefix every row sees keys
 template <int HD, int JW>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __restrict__ o_part, const float2* __restrict__ ml, long long rows,
-                                                                int parts, int H, bf16_t* __restrict__ out, int ldo) {
+                                                                int parts, int H, bf16_t* __restrict__ out, int ldo, const JoinSees v) {
     constexpr int LPR = HD / 4, RPB = 256 / (LPR * JW);  // threads of a row's channels, rows of a workgroup
     const int c = threadIdx.x % LPR, w = (threadIdx.x / LPR) % JW, lr = threadIdx.x / (LPR * JW);
     const long long row = (long long)blockIdx.x * RPB + lr;
@@ -1362,7 +1371,14 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __r
 #pragma unroll
         for (int k = 1; k < JW; ++k) join_part(M, L, o, sl[threadIdx.x + k * LPR].x, sl[threadIdx.x + k * LPR].y, so[threadIdx.x + k * LPR]);
     }
-    if (on) store_row_quad(out + (size_t)(row / H) * ldo + (row % H) * HD + 4 * c, L, o);
+    if (!on) return;
+    const int token = (int)(row / H);
+    bool sees = v.prefix != 0;
+    if (L == 0.f && !sees) {
+        const int n = rows_of_slot(v.kv_lens, v.kv_len, v.rows, token / v.T);
+        sees = (v.causal ? n - v.T + token % v.T + 1 : n) > 0;
+    }
+    store_row_quad(out + (size_t)token * ldo + (row % H) * HD + 4 * c, L, sees, o);
 }
 
 __global__ void kv_zero_kernel(unsigned* p, int n) {
@@ -1595,10 +1611,10 @@ static void launch_blocks(const AttnArgs& a, int block_rows, unsigned blocks, hi
 }
 
 template <int HD, int JW>
-static void launch_join(const AttnArgs& a, const KvPlan& pl, hipStream_t s) {
+static void launch_join(const AttnArgs& a, const KvPlan& pl, const JoinSees& v, hipStream_t s) {
     constexpr int RPB = 256 / (HD / 4 * JW);
     hipLaunchKernelGGL((kv_attention_join_kernel<HD, JW>), dim3((unsigned)((pl.rows + RPB - 1) / RPB)), dim3(256), 0, s, a.o_part, a.ml_part,
-                       pl.rows, pl.parts, a.H, a.out, a.ldo);
+                       pl.rows, pl.parts, a.H, a.out, a.ldo, v);
 }
 
 template <int HD, bool MX>
@@ -1622,8 +1638,9 @@ static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, c
         }
     }
     if (pl.parts > 1 && !pl.units) {
-        if (pl.parts > 4) launch_join<HD, 8>(a, pl, s);
-        else launch_join<HD, 1>(a, pl, s);
+        const JoinSees v = {kv_lens, kv_len, own.rows, a.T, a.causal, prefix_len};
+        if (pl.parts > 4) launch_join<HD, 8>(a, pl, v, s);
+        else launch_join<HD, 1>(a, pl, v, s);
     }
 }
 

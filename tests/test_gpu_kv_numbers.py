@@ -1,5 +1,5 @@
 """Attention over KV caches on the GPU where its numbers are at their edges: how the weights are normalised, tails of small weights, scores far
-beyond those of a trained model.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
+beyond those of a trained model, scores of minus infinity.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
 import math
 
 import pytest
@@ -142,3 +142,42 @@ def test_scores_of_billions_behind_a_prefix_and_over_split_keys(T):
         out = KVAttention(_cache(k, v, BF), heads=1, tokens=T, scale=0.127, prefix=_cache(pk, pv, BF), prefix_len=P)(q, n).cpu().double()
         want = torch.stack(rows).double().mean(0)
         assert ((out - want).abs() <= (len(rows) - 1) * _half(BF) * 1.01 * want.abs()).all()
+
+
+# ------------------------------------------------------------------------------------------------ minus infinity
+@pytest.mark.parametrize("T", ROWS)
+def test_rows_whose_scores_are_all_minus_infinity(T):
+    """The softmax of them is 0 / 0: NaN, as the formula gives it; one finite score among them takes all; a query that sees no row at all gets
+    zeros."""
+    D = 128
+    n = (T + 1) // 2                                                               # causal: the first T - n queries see nothing
+    k = torch.zeros(1, n, D)
+    k[:, :, 0] = -math.inf
+    v = torch.randn(1, n, D, generator=torch.Generator().manual_seed(6)).to(BF)
+    q = torch.ones(T, D, dtype=BF).cuda()
+    out = KVAttention(_cache(k, v, BF, n + 40), heads=1, tokens=T)(q, n).cpu()
+    assert (out[:T - n] == 0).all() and torch.isnan(out[T - n:]).all()
+    assert (KVAttention(_cache(k, v, BF, n + 40), heads=1, tokens=T)(q, 0) == 0).all()
+    k[0, 0, 0] = 0.0
+    out = KVAttention(_cache(k, v, BF, n + 40), heads=1, tokens=T)(q, n).cpu()
+    assert (out[:T - n] == 0).all() and torch.equal(out[T - n:], v[0, :1].expand(n, D))
+
+
+@pytest.mark.parametrize("T", ROWS)
+def test_minus_infinity_behind_a_prefix_and_over_split_keys(T):
+    D, n, P = 128, 700, 900
+    k, pk = torch.zeros(1, n, D), torch.zeros(1, P, D)
+    k[:, :, 0] = pk[:, :, 0] = -math.inf
+    v, pv = (torch.randn(1, r, D, generator=torch.Generator().manual_seed(r)).to(BF) for r in (n, P))
+    q = torch.ones(T, D, dtype=BF).cuda()
+
+    def attend(k, pk, held):
+        return KVAttention(_cache(k, v, BF), heads=1, tokens=T, prefix=_cache(pk, pv, BF), prefix_len=P)(q, held).cpu()
+    assert torch.isnan(attend(k, pk, n)).all() and torch.isnan(attend(k, pk, 0)).all()
+    assert torch.isnan(KVAttention(_cache(k, v, BF), heads=1, tokens=T)(q, n)).all()
+    pk[0, 444, 0] = 0.0
+    assert torch.equal(attend(k, pk, n), pv[0, 444:445].expand(T, D)) and torch.equal(attend(k, pk, 0), pv[0, 444:445].expand(T, D))
+    pk[0, 444, 0] = -math.inf
+    k[0, 5, 0] = 0.0
+    assert torch.equal(attend(k, pk, n), v[0, 5:6].expand(T, D))
+    assert torch.equal(KVAttention(_cache(k, v, BF), heads=1, tokens=T)(q, n).cpu(), v[0, 5:6].expand(T, D))
