@@ -314,7 +314,7 @@ int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int
  * n_b = kv_len rows, or kv_lens_i32[b] + kv_len where kv_lens_i32 (device int32 [B]) is given - kv_len = T with the lengths that
  * seedmi_kv_append took, 0 with lengths that count the new rows already - and none where kv_lens_i32[b] is negative (idle).  The T queries
  * are the slot's last rows: with causal != 0 query t sees rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all
- * visible) rows 0 .. n_b - 1.  n_b is clamped to [0, cache->rows]; scale is finite and above 0.  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
+ * visible) rows 0 .. n_b - 1.  n_b is clamped to [0, cache->rows]; scale is above 0 and at most 2.3e38 (scale log2 e is finite).  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
  * head_dim), in front of its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros, one whose
  * scores are all -infinity NaN.
  * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the

@@ -4,6 +4,7 @@
 //                       length per slot
 //  seedmi_kv_read       8-bit rows back as 16-bit tensors
 //  seedmi_kv_attention  memory_efficient_attention over the cache (llama_xformer.py:244-256), optionally behind a prefix that all slots share
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 #include <string.h>
@@ -1644,6 +1645,8 @@ static void launch_attention(AttnArgs a, const KvView& own, const KvView& pre, c
     }
 }
 
+constexpr float LOG2E = 1.44269504088896340736f;
+
 int seedmi_kv_attention_impl(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq, void* out,
                              int ldo, int B, int T, int H, int kv_len, const void* kv_lens_i32, int kv_max, float scale, int causal,
                              void* workspace, size_t workspace_bytes, void* stream, bool launch) {
@@ -1664,9 +1667,9 @@ int seedmi_kv_attention_impl(const seedmi_kv_cache_t* cache, const seedmi_kv_cac
         }
     }
     if (!q || !out || B <= 0 || B > cache->slots || T <= 0 || H <= 0 || (H % G) || ldq < (long long)H * hd || ldo < (long long)H * hd ||
-        kv_max < 0 || !(scale > 0.f) || scale > 3e38f) {
+        kv_max < 0 || !(scale > 0.f) || !(scale * LOG2E <= FLT_MAX)) {
         seedmi_set_error("seedmi_kv_attention: null pointer or bad shape: B=%d (slots %d) T=%d H=%d (a multiple of %d) ldq=%d ldo=%d kv_max=%d "
-                         "scale=%g (finite, above 0)", B, cache->slots, T, H, G, ldq, ldo, kv_max, scale);
+                         "scale=%g (above 0, finite in base-2 exponents: at most 2.3e38)", B, cache->slots, T, H, G, ldq, ldo, kv_max, scale);
         return SEEDMI_E_SHAPE;
     }
     if (kv_len < 0 || kv_len > cache->rows) {
@@ -1691,7 +1694,7 @@ int seedmi_kv_attention_impl(const seedmi_kv_cache_t* cache, const seedmi_kv_cac
     a.q = (const bf16_t*)q;
     a.out = (bf16_t*)out;
     a.ldq = ldq; a.ldo = ldo; a.T = T; a.H = H; a.GH = H / G;
-    a.causal = causal; a.c2 = scale * 1.44269504088896340736f;
+    a.causal = causal; a.c2 = scale * LOG2E;
     a.rows = pl.rows; a.parts = pl.parts;
     a.arrivals = pl.units ? (unsigned*)workspace : nullptr;
     a.unit_blocks = pl.unit_blocks; a.unit_rows = pl.unit_rows;

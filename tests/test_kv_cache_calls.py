@@ -199,3 +199,12 @@ def test_a_short_attention_workspace_is_refused_before_anything_runs():
     assert need > 0
     for ws, n in ((None, 0), (FAKE, need - 1), (FAKE + 128, need)):
         assert _forward_kv(kv, B=1, T=1, past_max=4000, aws=ws, ab=n) == -3
+
+
+# ------------------------------------------------------------------------------------------------ scale
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("inf"), float("nan"), 3.3e38, 2.5e38])
+def test_scales_that_are_not_finite_in_base_2_exponents_are_refused(scale):
+    """2.5e38 log2 e is beyond fp32: every score would be infinite, or NaN where it is 0."""
+    h = _handle()
+    rc = L.load().seedmi_kv_attention(C.byref(h), None, 0, FAKE, 256, FAKE, 256, 4, 1, 2, 8, None, 0, scale, 1, None, 0, None)
+    assert rc == -1 and "scale" in L.load().seedmi_last_error().decode()
