@@ -306,7 +306,8 @@ SEEDMI_DEVINL bool bad_words(const uint4& w) { return bad_word(w.x) | bad_word(w
 SEEDMI_DEVINL uint32_t clean_word(uint32_t w) { return (bad16(w) ? 0u : w & 0xffffu) | (bad16(w >> 16) ? 0u : w & 0xffff0000u); }
 
 // The rows 0 .. n - 1 of a (slot, head) as buffers: a load takes a per-lane offset that never changes and a scalar one for the tile, and
-// rows from n on read as zeros without touching memory.
+// rows from n on read as zeros without touching memory.  (The scalar offset counts in the range check, a load whose scalar offset alone is at
+// or beyond the end included - the requests for a tile behind the last one: tools/probes/buffer_range_probe.hip, every size of load.)
 struct RowBuffers { __amdgpu_buffer_rsrc_t k, v, ks, vs; };
 template <int HD, bool MX>
 SEEDMI_DEVINL RowBuffers row_buffers(const KvView& c, long long row0, int n) {
