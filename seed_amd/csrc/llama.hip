@@ -1779,6 +1779,10 @@ extern "C" int seedmi_gemm_skinny_ws_status(void* workspace, size_t workspace_by
     return SEEDMI_E_HIP;
 }
 
+static __global__ void clear_words_kernel(unsigned* p, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0u;
+}
+
 // Once after allocation: hand-off flags and error word zero, tag set (stream-ordered; no synchronisation)
 extern "C" int seedmi_gemm_skinny_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
     if (!workspace || workspace_bytes < SK2_WS_BYTES || ((uintptr_t)workspace & 255)) {
@@ -1950,9 +1954,9 @@ static int llama_forward_impl(const seedmi_llama_weights_t* w, const void* ids_i
 #else
     void* const gsk = nullptr;
 #endif
-    if (sk && !fused_first && hipMemsetAsync(sk, 0, SK2_LIVE_WORDS * 4, (hipStream_t)stream) != hipSuccess) {     // (the kernels leave the
-        seedmi_set_error("seedmi_llama_forward: clearing the split-K flag words failed");                       //  words zero: safety net)
-        return SEEDMI_E_HIP;
+    if (sk && !fused_first) {                            // (the kernels leave the words zero: safety net; a kernel, so that a captured call
+        hipLaunchKernelGGL(clear_words_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, (unsigned*)sk, SK2_LIVE_WORDS);    // records no memset node)
+        CK(seedmi_check_launch("llama_clear_flags"));
     }
     if (fold && !fused_first) CK(seedmi_pack_activations_bf16(t.x, h, t.xn, M, h, stream));
     int mega_done = 0;

@@ -134,3 +134,25 @@ def test_new_workspaces_of_forward_kv_are_ready_for_any_stream(engine):
     torch.cuda.synchronize()
     for got, x, n, most in ((first, ids, 0, 0), (second, tok, 30, 240), (third, tok, 31, 240)):
         assert torch.equal(got, engine.forward_kv(x, twin, _lens(n, n), most))
+
+
+@pytest.mark.parametrize("fold", [True, False])
+def test_a_captured_step_replays_with_and_without_folded_norms(fold):
+    """Without folded norms the step clears the split-K flags itself: replays with eager steps and synchronisations between them."""
+    eng = LlamaEngine(make_llama_state_dict(CFG, seed=11, norm_jitter=0.1), CFG, device="cuda", batch_cap=4, tmax=128, fold_norm=fold)
+    kv, twin = eng.new_kv(2, 250), eng.new_kv(2, 250)
+    tok, past = torch.tensor([[5], [7]]).cuda(), _lens(0, 0)
+    step = lambda c: eng.forward_kv(tok, c, past, 200, last_only=True)  # noqa: E731
+    step(kv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(kv)
+    for i in range(6):
+        tok.fill_(11 + i)
+        graph.replay()
+        want = step(twin)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        past += 1
+    eng.decode_status(2)
