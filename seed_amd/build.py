@@ -21,8 +21,8 @@ DEVTOOLS_CSRC = os.path.join(os.path.dirname(HERE), "tools", "devtools_csrc")
 LIB_F16 = os.path.join(HERE, "libseedmi_f16.so")          # the same sources with -DSEEDMI_F16: IEEE fp16 as the 16-bit element (csrc/common.h)
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["capi.hip", "gemm_bf16.hip", "attn_fullrow.hip", "attn_vit.hip", "norm_misc.hip", "vq_argmin.hip", "tokenizer.hip", "detokenizer.hip", "preprocess.hip", "sample.hip", "llama.hip", "kv_cache.hip"]
-# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware now and then; same
-# tokenize and decode rates without them (2116 / 2115 images/s).  The host pass does not know the feature and says so: harmless.
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): which sums and products the compiler pairs would decide what it fuses, and with it
+# last bits; same tokenize and decode rates without them (2116 / 2115 images/s).  The host pass does not know the feature and says so: harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-unused-result",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -36,17 +36,35 @@ def _deps_mtime():
     return latest
 
 
+def _read(path):
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _older(lib, objs):
+    """The library is missing, or older than an object of it (a link that failed after its objects were built)."""
+    return not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs)
+
+
 def _compile(src, force, objdir=OBJ, extra=()):
     obj = os.path.join(objdir, src.replace(".hip", ".o"))
     srcp = os.path.join(CSRC, src)
     hdr_m = max(os.path.getmtime(os.path.join(d, f)) for d in (CSRC, DEVTOOLS_CSRC) if os.path.isdir(d) for f in os.listdir(d) if f.endswith((".h", ".inc")))
     hdr_m = max(hdr_m, os.path.getmtime(os.path.join(os.path.dirname(HERE), "include", "seedmi.h")))
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(srcp), hdr_m):
-        return obj, False
     cmd = [HIPCC] + FLAGS + list(extra) + ["-c", srcp, "-o", obj]
+    stamp = obj + ".cmd"                                  # the command the object was built with: other flags make it out of date too
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(srcp), hdr_m) and _read(stamp) == "\n".join(cmd):
+        return obj, False
+    if os.path.exists(stamp):
+        os.remove(stamp)                                  # (a build that fails or is interrupted leaves an object that counts as out of date)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write("\n".join(cmd))
     return obj, True
 
 
@@ -58,7 +76,7 @@ def build_variant(name: str, defines, verbose: bool = True) -> str:
     with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
         results = list(ex.map(lambda s: _compile(s, False, objdir, tuple(defines)), SOURCES))
     objs = [o for o, _ in results]
-    if any(changed for _, changed in results) or not os.path.exists(lib):
+    if any(changed for _, changed in results) or _older(lib, objs):
         r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib] + objs, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
@@ -82,7 +100,7 @@ def build(force: bool = False, verbose: bool = True, devtools: bool = False, f16
         results = list(ex.map(lambda s: _compile(s, force, objdir, extra), SOURCES))
     objs = [o for o, _ in results]
     LIB_ = lib
-    if any(changed for _, changed in results) or not os.path.exists(LIB_) or force:
+    if any(changed for _, changed in results) or _older(LIB_, objs) or force:
         cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_] + objs
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

@@ -13,9 +13,16 @@ _lib = None
 def build(force=False):
     src = os.path.join(HERE, "calib.hip")
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(HERE, "seedcal.h")))
-    if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
-        subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-                               "-shared", "-fPIC", "-o", LIB, src])
+    cmd = [HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC",
+           "-o", LIB, src]
+    stamp = LIB + ".cmd"                                  # built with other flags: out of date
+    if not force and os.path.exists(stamp) and os.path.exists(LIB) and os.path.getmtime(LIB) >= newest:
+        with open(stamp) as f:
+            if f.read() == "\n".join(cmd):
+                return LIB
+    subprocess.check_call(cmd)
+    with open(stamp, "w") as f:
+        f.write("\n".join(cmd))
     return LIB
 
 
