@@ -1,11 +1,12 @@
 """Attention over KV caches on the GPU where its numbers are at their edges: how the weights are normalised, tails of small weights, scores far
-beyond those of a trained model, scores of minus infinity.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
+beyond those of a trained model, scores of minus infinity; the 8-bit format over all codes and values.  Every kernel: 1 - 32, 33 - 128 and more query rows per key head."""
 import math
 
 import pytest
 import torch
 
 from seed_amd.kv_cache import KVAttention, KVCache
+from tests import _kv_ref as R
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +182,36 @@ def test_minus_infinity_behind_a_prefix_and_over_split_keys(T):
     k[0, 5, 0] = 0.0
     assert torch.equal(attend(k, pk, n), v[0, 5:6].expand(T, D))
     assert torch.equal(KVAttention(_cache(k, v, BF), heads=1, tokens=T)(q, n).cpu(), v[0, 5:6].expand(T, D))
+
+
+# ------------------------------------------------------------------------------------------------ the 8-bit format, value by value
+def _same(got, want):
+    return torch.equal(torch.where(torch.isnan(want), torch.zeros_like(want), want).view(torch.int16),
+                       torch.where(torch.isnan(got), torch.zeros_like(got), got).view(torch.int16)) and torch.equal(torch.isnan(want), torch.isnan(got))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_every_code_under_every_scale_byte_reads_back(dtype):
+    """256 codes x 254 scale bytes: code * 2^(byte - 127) rounded once to the element, subnormal results and overflows included, bit for bit."""
+    byte = torch.arange(1, 255, dtype=torch.uint8).repeat_interleave(2).view(-1, 1).repeat(1, 4)
+    code = torch.arange(256, dtype=torch.uint8).view(2, 128).repeat(254, 1)
+    cache = KVCache.new(1, 1, 508, 128, "mx8", dtype)
+    cache.k[0, 0], cache.k_scale[0, 0] = code.cuda(), byte.cuda()
+    k, _ = cache.read(0, 508)
+    assert _same(k[0, 0].cpu(), R.mx_decode(code, byte).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("order", ["alike", "mixed"])
+def test_every_16_bit_value_is_stored_by_the_formula(dtype, order):
+    """All 65536 bit patterns as values of a cache, 32 neighbours to a block or 32 of all magnitudes: codes and scale bytes bit for bit (a NaN's
+    code by its being one)."""
+    x = torch.arange(1 << 16, dtype=torch.int32)
+    x = (x if order == "alike" else x.view(32, -1).t().reshape(-1)).to(torch.int16).view(dtype).view(-1, 128)
+    cache = KVCache.new(1, 1, 512, 128, "mx8", dtype)
+    one = torch.ones(512, 128, dtype=dtype).cuda()
+    cache.append(torch.cat((torch.zeros(512, 256, dtype=dtype), x), 1).cuda(), one, one * 0, 0, heads=1)
+    code, byte = R.mx_encode(x, R.top(dtype))
+    got, nan = cache.v[0, 0].cpu(), (code & 127) == 127
+    assert torch.equal(cache.v_scale[0, 0].cpu(), byte)
+    assert torch.equal(got[~nan], code[~nan]) and ((got[nan] & 127) == 127).all()
