@@ -317,8 +317,8 @@ __global__ __launch_bounds__(64 * VWAVES) void attn_vit_kernel(VitAttnParams p) 
 // waits 6-10 k of a 31.6 k cycle item).  Here every wave owns exactly one tile (4 waves per SIMD, 128 registers each), so a phase lasts
 // one tile's time with four waves interleaving on each SIMD, and the 17th tile - a single valid row - costs one wave a fraction of a tile:
 //   * its scores are formed with the operands SWAPPED (S = Q K^T instead of S^T = K Q^T): the accumulator then holds row 256 as ONE value
-//     per key tile in lanes 0..15 (key = 16 kt + lane), i.e. 17 values per lane instead of 68, and the softmax of that row is ~110
-//     VALU instructions on 16 lanes instead of ~450 on 64 (same arithmetic and rounding points; the reductions run over the 16 lanes);
+//     per key tile in lanes 0..15 (key = 16 kt + lane), i.e. 17 values per lane instead of 68, and the softmax of that row is about a
+//     quarter of the VALU instructions, on 16 lanes instead of 64 (same arithmetic and rounding points; the reductions run over the 16 lanes);
 //   * the normalised row goes to LDS as 272 halves; after the phase barrier ANOTHER wave (another SIMD) reads it back in the PV operand
 //     layout (every lane group g reads keys 32 kk + 4 g .. + 3 and + 16: a broadcast) and runs the ordinary PV for it.
 // The two side jobs rotate over the waves item by item.  Same arithmetic and rounding points as attn_vit_kernel / attn_fullrow.hip.
@@ -333,9 +333,8 @@ constexpr int V16_LDS_BYTES = VLDS_BYTES + 1024;
 //      bit 1: softmax normalisation moved behind PV.  P leaves the exponential UN-normalised (e = 2^((s - max) log2 e) <= 1, rounded to half)
 //             and the row sum comes out of the PV MFMAs themselves: the V image's 89th column (first pad column, never loaded: the staging
 //             skips the pad chunk) holds 1.0, so O^T row 88 = sum_k half(e_k) - exactly the sum of the values that were multiplied.
-//             O = O' / that sum: 24 multiplies instead of a 68-term sum, 68 multiplies and the reduction shuffles per tile; the exponent
-//             arguments are formed two at a time (v_pk_fma_f32).  ~270 instead of ~450 VALU instructions per tile, and the phase that
-//             holds them is VALU-bound.  This MOVES a rounding point: the reference rounds the normalised probabilities to half before PV
+//             O = O' / that sum: 24 multiplies instead of a 68-term sum, 68 multiplies and the reduction shuffles per tile, in a phase that
+//             is VALU-bound.  This MOVES a rounding point: the reference rounds the normalised probabilities to half before PV
 //             (eva_vit.py:153-156 under autocast), here the un-normalised ones are rounded and the quotient is formed in fp32 - the same
 //             relative rounding error per term, normalised consistently; results differ from the other kernels in the last half ulp.
 template <bool ROUND_S, int MODE>
@@ -499,7 +498,7 @@ __global__ __launch_bounds__(64 * V16_WAVES) void attn_vit16_kernel(VitAttnParam
             float sum = 0.f;                                 // (one chain in (kt, r) order, like the 12-wave kernel: bit-identical rows)
 #pragma unroll
             for (int kt = 0; kt < VNT; ++kt) {
-                // (exponent arguments two at a time - v_pk_fma_f32 - the same fma per element)
+                // (written two at a time, one fma per element)
                 const f32x2 a0 = __builtin_elementwise_fma((f32x2){s[kt][0], s[kt][1]}, (f32x2){L2E, L2E}, (f32x2){nmx, nmx});
                 const f32x2 a1 = __builtin_elementwise_fma((f32x2){s[kt][2], s[kt][3]}, (f32x2){L2E, L2E}, (f32x2){nmx, nmx});
                 const float arg[4] = {a0[0], a0[1], a1[0], a1[1]};

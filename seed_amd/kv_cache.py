@@ -153,7 +153,8 @@ class KVCache:
                pos_ids: Optional[torch.Tensor] = None, pos_base: int = 0, tokens: Optional[int] = None,
                q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """RoPE on the new rows' queries and keys, keys and values into the cache behind the ``past`` rows that each slot holds; returns the
-        rotated queries [rows, heads * head_dim].  ``qkv`` [slots * T, (heads + 2 kv_heads) * head_dim] (q | k | v), slot-major; ``cos`` /
+        rotated queries [rows, heads * head_dim].  ``qkv`` [slots * T, (heads + 2 kv_heads) * head_dim] (q | k | v), slot-major, T = ``tokens``
+        or, without it, what the rows divide into over the slots that ``past`` lists (all slots for an int); ``cos`` /
         ``sin`` [positions, head_dim] in the cache's type; positions are ``pos_ids`` (int64 [slots * T]) or pos_base + past + t."""
         D = self.head_dim
         heads, pos_base = L.int32("KVCache.append: heads", heads), L.int32("KVCache.append: pos_base", pos_base)
@@ -260,9 +261,10 @@ class KVAttention:
         self._fn, self._rows, self._cols = cache.lib.seedmi_kv_attention, self.slots * tokens, heads * cache.head_dim
 
     def __call__(self, q: torch.Tensor, kv_len: Lengths, out: Optional[torch.Tensor] = None, plus: int = 0) -> torch.Tensor:
-        """q [slots * tokens, heads * head_dim] -> out of the same shape; ``kv_len``: rows each slot holds, the query rows' own included
-        (an int, or an int32 tensor with one entry per slot; 0 or less for an idle slot).  ``plus`` is added to a tensor's entries that are not
-        negative: ``attention(q, past, plus=T)`` takes the lengths that ``append`` took.  Queries that see nothing get zeros."""
+        """q [slots * tokens, heads * head_dim] -> out of the same shape; ``kv_len``: rows each slot holds, the query rows' own included: an
+        int of 0 or more, or an int32 tensor with one entry per slot, 0 or less for an idle one.  ``plus`` is added to an int and to a tensor's
+        entries that are not negative: ``attention(q, past, plus=T)`` takes the lengths that ``append`` took.  Queries that see nothing get
+        zeros."""
         c, cols, rows = self.cache, self._cols, self._rows
         ldq = c._rows_of("KVAttention", q, cols)
         if q.size(0) != rows:
