@@ -266,7 +266,9 @@ SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, w), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), acc, false);
 #endif
 }
-// The sum of a row is that of its probabilities as they are rounded for the product with the values: out is then a mean of the values with
+// Probabilities are rounded to the element for the product with the values, whose matrix instructions take operands of one type: in bf16 the
+// error against 64 bits is 0.0017 - 0.0019 relative, 0.0016 - 0.0018 of it the output's own rounding (fp16: 0.00022, 0.00021).
+// The sum of a row is that of its probabilities as they are rounded: out is then a mean of the values with
 // weights that add up to one, in every kernel.  (A sum of unrounded ones is off by what the roundings have in common: 387 equal scores of 400
 // made every output 0.92 half steps of the type too small.)
 SEEDMI_DEVINL float add_probabilities(const uint4& w, float acc) { return add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, acc)))); }
@@ -525,8 +527,8 @@ SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh,
 
 // ---- few query rows per group (decode, drafted tokens, a shared prefix): bound by the bytes of the cache.
 // Bytes: 2 rows of HD values per key and key head, once; 4 HD flops per (row, key) are far below what they cost up to some 100 rows.
-// 32 x 32 heads: 4096 rows each 186 us (8-bit, 6.0 TB/s) / 356 us (16-bit, 6.0); slots of different lengths up to 2048
-// rows 68 us (5.2); 4 x 8 heads of 23 - 65 thousand rows 82 us (4.6, with the parts' join); one conversation of 700 rows 8.3 us, latency.
+// 32 x 32 heads: 4096 rows each 183 us (8-bit, 6.05 TB/s) / 355 us (16-bit, 6.05); slots of different lengths up to 2048
+// rows 69 us (5.1); 4 x 8 heads of 23 - 65 thousand rows 82 - 89 us (4.6 - 4.2, with the parts' join); one conversation of 700 rows 8.4 us, latency.
 // Workgroup = (group, block of 16 MT rows, key range); its 4 waves take the range's tiles in turn, each with a running softmax of its own,
 // and join at the end (eight waves: 4 slots of 65 thousand rows 85 -> 81 us, one short conversation 8.3 -> 9.2).
 // S^T = K Q^T (keys are the MFMA's rows: K fragments come straight from memory, one tile ahead in registers), so a
@@ -768,7 +770,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : MX ? 4 : 3) void kv_attention_fe
 // ---- many query rows per group (prompt chunks, a prefix that many slots share): bound by the matrix and vector pipes.
 // Workgroup = (group, block of 64 MT rows, key range), wave = 16 MT rows; 64-key tiles of K and V are widened to 16 bits once and shared
 // through a double-buffered LDS image, one barrier per tile; the next tile's bytes are in registers meanwhile, so that neither the load nor
-// the widening sits between two tiles.  8 x 40 heads, 100 new rows behind 549: 40 us (8-bit) / 38 us (16-bit).
+// the widening sits between two tiles.  8 x 40 heads, 100 new rows behind 549: 40 us (8-bit) / 37 us (16-bit).
 constexpr int KT2 = 64;
 
 template <int HD, bool MX>
@@ -1026,8 +1028,8 @@ __global__ __launch_bounds__(256, 2) void kv_attention_many_kernel(const AttnArg
 // values of t + h - two LDS buffers each, always written after their last reader's barrier.
 // Tiles that every row of the block sees whole take a loop without masks and case distinctions (a lone wave issues an instruction every
 // five to six cycles, scalar ones too: it is their number that counts).
-// 2 x 32 heads, 2048 new rows each in caches of up to 4001: 138 GF in 192 us, 717 TFLOP/s (both slots at 4001 rows: 238 us, 839); a plain
-// 8192^3 product of the type reaches 1284.  With one phase's work taken out (kernel at 195 us): matrix phases alone 135 us, vector phases
+// 2 x 32 heads, 2048 new rows each in caches of up to 4001: 138 GF in 192 - 196 us, 717 - 703 TFLOP/s (both slots at 4001 rows: 246 us, 811); a
+// plain 8192^3 product of the type reaches 1284 and more.  With one phase's work taken out (kernel at 195 us): matrix phases alone 135 us, vector phases
 // alone 162; without the requests for the next tiles 160.
 // On 16 x 16 x 32 products and one loop for all tiles the same kernel took 232 us, unphased with two workgroups per CU 244.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
