@@ -156,3 +156,143 @@ def test_a_captured_step_replays_with_and_without_folded_norms(fold):
         assert torch.equal(out, want), i
         past += 1
     eng.decode_status(2)
+
+
+# ------------------------------------------------------------------------------------------------ calls together, captured, at the largest sizes
+def _filled(B, G, rows, D, fmt, dtype, seed):
+    c = KVCache.new(B, G, rows, D, fmt, dtype)
+    for i, (x, s) in enumerate(((c.k, c.k_scale), (c.v, c.v_scale))):
+        v = _rand((B, G, rows, D), dtype, seed + i)
+        if fmt == "16":
+            x.copy_(v)
+        else:
+            code, byte = R.mx_encode(v, R.top(dtype))
+            x.copy_(code)
+            s.copy_(byte)
+    return c
+
+
+def test_two_objects_and_a_graph_over_one_cache_at_the_same_time():
+    """Two streams and a replaying graph, an object each, 30 calls in flight: every output as it is alone."""
+    H, G, D, B, P = 8, 2, 128, 3, 900
+    cache, prefix = _filled(B, G, 2000, D, "mx8", BF, 1), _filled(1, G, P, D, "mx8", BF, 5)
+    lens = _lens(2000, 700, 1)
+    make = [lambda: KVAttention(cache, heads=H), lambda: KVAttention(cache, heads=H, prefix=prefix, prefix_len=P),
+            lambda: KVAttention(cache, heads=H, tokens=20, prefix=prefix, prefix_len=P)]
+    qs = [_rand((B * t, H * D), BF, 7 + t).cuda() for t in (1, 1, 20)]
+    want = [m()(q, lens) for m, q in zip(make, qs)]
+    attns = [m() for m in make]
+    assert all(a.workspace is not None for a in attns)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attns[2](qs[2], lens)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for s, a, q, g in zip(streams, attns, qs, got):
+            with torch.cuda.stream(s):
+                g.append(a(q, lens))
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[2])
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
+
+
+@pytest.mark.parametrize("T,P", [(20, 0), (60, 700), (300, 0), (200, 900)])
+def test_captured_chunks_replay_with_new_lengths(T, P):
+    """append and attention of more than one token per slot, with parts that a launch of its own joins, replayed as the lengths grow."""
+    H, G, D, B, rows = 4, 2, 128, 2, 1700
+    cos, sin = (_rand((4096, D), BF, 3 + i).clamp(-1, 1).cuda() for i in range(2))
+    prefix = _filled(1, G, P, D, "mx8", BF, 30) if P else None
+    cache, twin = _filled(B, G, rows, D, "mx8", BF, 9), _filled(B, G, rows, D, "mx8", BF, 9)
+    make = lambda c: KVAttention(c, heads=H, tokens=T, prefix=prefix, prefix_len=P)  # noqa: E731
+    attn, other = make(cache), make(twin)
+    past, qkv, q = _lens(500, 3), torch.zeros(B * T, (H + 2 * G) * D, dtype=BF).cuda(), torch.empty(B * T, H * D, dtype=BF).cuda()
+    out = torch.empty_like(q)
+
+    def step():
+        cache.append(qkv, cos, sin, past, heads=H, pos_base=P, q_out=q)
+        attn(q, past, plus=T, out=out)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        qkv.copy_(_rand(qkv.shape, BF, 60 + i).cuda())
+        graph.replay()
+        want = other(twin.append(qkv, cos, sin, past, heads=H, pos_base=P), past, plus=T)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        past += T
+
+
+@pytest.mark.parametrize("fmt", ["16", "mx8"])
+@pytest.mark.parametrize("T", [1, 20, 60, 100, 300])
+def test_the_longest_cache(fmt, T):
+    """2^22 rows, the most that a cache may have: queries that single out four keys far apart, 30 ahead of the others, which have e^-30 2^22 <
+    5e-7 of the sum together.  Tolerance: output and probabilities half a step each, scores of 30 to 2^-17, sums of at most 2^16 terms in
+    a row."""
+    D, n = 128, 1 << 22
+    at = torch.tensor([0, n // 2 + 3, n - 70, n - 1])
+    dt = BF if fmt == "16" else torch.uint8
+    k, v = (torch.zeros(1, 1, n, D, dtype=dt, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((1, 1, n, D // 32), 127, dtype=torch.uint8, device="cuda") if fmt == "mx8" else None for _ in range(2))
+    key = torch.zeros(4, D)
+    key[:, 0] = torch.tensor([30.0, 32.0, 30.0, 32.0])
+    val = _rand((4, D), BF, 2)
+    if fmt == "16":
+        k[0, 0, at.cuda()], v[0, 0, at.cuda()] = key.to(BF).cuda(), val.cuda()
+        vals = val.double()
+    else:
+        for x, s, y in ((k, ks, key.to(BF)), (v, vs, val)):
+            code, byte = R.mx_encode(y, R.top(BF))
+            x[0, 0, at.cuda()], s[0, 0, at.cuda()] = code.cuda(), byte.cuda()
+        vals = R.mx_decode(*R.mx_encode(val, R.top(BF)))
+    q = torch.zeros(T, D)
+    q[:, 0] = 1.0
+    cache = KVCache.wrap(k, v, ks, vs, dtype=BF)
+    out = KVAttention(cache, heads=1, tokens=T, scale=1.0, causal=False)(q.to(BF).cuda(), n).cpu().double()
+    w = torch.softmax(key[:, 0].double(), 0)
+    want, u = w @ vals, 2.0 ** -8
+    tol = 1.01 * u * want.abs() + (1.02 * u + 2.0 ** -15 + 2 * 65536 * 2.0 ** -24) * (w @ vals.abs()) + 5e-7
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() - tol).max().item()
+
+
+def test_read_of_values_alone_and_append_of_the_first_slots():
+    """seedmi_kv_read with one output; append with tokens= on fewer slots than there are lengths."""
+    H, D, dtype = 2, 128, BF
+    cache = _filled(4, H, 40, D, "mx8", dtype, 3)
+    both = cache.read(5, 7)
+    for i in range(2):
+        out = torch.zeros_like(both[0])
+        p = [None, None]
+        p[i] = out.data_ptr()
+        L.check(cache.lib.seedmi_kv_read(cache._ref, p[0], p[1], 4, 7, 5, None, L.stream_ptr()), "read", cache.lib)
+        assert torch.equal(out, both[i])
+    before = cache.k.clone()
+    cos, sin = (_rand((64, D), dtype, 4 + i).cuda() for i in range(2))
+    cache.append(_rand((6, 3 * H * D), dtype, 8).cuda(), cos, sin, _lens(1, 30, 9, 9), heads=H, tokens=3)
+    changed = (cache.k != before).any(-1).any(1).cpu()
+    assert changed[0, 1:4].all() and changed[1, 30:33].all() and int(changed.sum()) == 6
+
+
+@pytest.mark.parametrize("B", [40, 70])
+def test_more_slots_than_the_static_cache_has(B, engine):
+    """One step of 40 and of 70 slots (the engine's own cache has 4): each slot's logits as in a call of four."""
+    kv = engine.new_kv(B, 20, "16")
+    ids = torch.randint(3, CFG.vocab, (B, 6), generator=torch.Generator().manual_seed(4)).cuda()
+    past = torch.zeros(B, dtype=torch.int32).cuda()
+    engine.forward_kv(ids[:, :5].contiguous(), kv, past, 0)
+    past += 5
+    got = engine.forward_kv(ids[:, 5:].contiguous(), kv, past, 5, last_only=True)
+    for b in range(0, B, 13):
+        one = engine.new_kv(1, 20, "16")
+        engine.forward_kv(ids[b:b + 1, :5].contiguous(), one, past[:1] * 0, 0)
+        want = engine.forward_kv(ids[b:b + 1, 5:].contiguous(), one, past[:1], 5, last_only=True)
+        d = (got[b].double() - want[0].double()).norm() / want[0].double().norm()
+        assert d.item() < 2e-2, (b, d.item())
