@@ -298,8 +298,8 @@ struct seedmi_kv_cache {
 typedef struct seedmi_kv_cache seedmi_kv_cache_t;
 /* seedmi_rope_kv_append for a cache handle: the rows of slots 0 .. B - 1 behind what each holds.  qkv [B*T, (H + 2 * kv_heads) * head_dim]
  * (q | k | v, row stride ldqkv); queries and keys are rotated as half(half(x cos) + half(rotate_half(x) sin)) (bf16: bit-identical to
- * seedmi_rope_kv_append; the fp16 build of that one fuses a product into the sum), queries go to q_out [B*T, H * head_dim] (row stride ldq), keys and values into cache rows n_b .. n_b + T - 1, where n_b = past_lens_i32[b]
- * (device int32 [B]) or past_len when that is NULL.  The position of row (b, t) is pos_ids_i64[b * T + t], or pos_base + n_b + t when that
+ * seedmi_rope_kv_append; the fp16 build of that one fuses a product into the sum), queries go to q_out [B*T, H * head_dim] (row stride ldq),
+ * keys and values into cache rows n_b .. n_b + T - 1, where n_b = past_lens_i32[b] (device int32 [B]) or past_len when that is NULL.  The position of row (b, t) is pos_ids_i64[b * T + t], or pos_base + n_b + t when that
  * is NULL (pos_base = the length of a shared prefix in front), clamped to [0, max_pos).  A slot whose device-resident length is negative is
  * idle: nothing is written to the cache for it; rows at or beyond cache->rows are not written.  The rows of different (slot, head) pairs
  * must not overlap. */
@@ -314,15 +314,17 @@ int seedmi_kv_read(const seedmi_kv_cache_t* cache, void* k_out, void* v_out, int
  * n_b = kv_len rows, or kv_lens_i32[b] + kv_len where kv_lens_i32 (device int32 [B]) is given - kv_len = T with the lengths that
  * seedmi_kv_append took, 0 with lengths that count the new rows already - and none where kv_lens_i32[b] is negative (idle).  The T queries
  * are the slot's last rows: with causal != 0 query t sees rows 0 .. n_b - T + t, otherwise (keys of an encoder, a prompt that is all
- * visible) rows 0 .. n_b - 1.  n_b is clamped to [0, cache->rows]; scale is above 0 and at most 2.3e38 (scale log2 e is finite).  With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and
- * head_dim), in front of its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros, one whose
- * scores are all -infinity NaN.
- * A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32; the
- * probabilities (unnormalised, 0 .. 1) are rounded to the 16-bit element for the product with the values.
+ * visible) rows 0 .. n_b - 1.  n_b is clamped to [0, cache->rows]; scale is above 0 and at most 2.3e38 (scale log2 e is finite).
+ * With prefix_len > 0 every query also sees rows 0 .. prefix_len - 1 of slot 0 of `prefix` (same format, kv_heads and head_dim), in front of
+ * its own rows: the prefix is read once for all slots when T is small.  A query that sees no row at all gets zeros, one whose scores are all
+ * -infinity NaN.  A row that a query does not see has no influence on it, whatever it holds.  Scores, softmax statistics and sums are fp32;
+ * the probabilities are rounded to the 16-bit element for the product with the values (fp16: times 2^15, so that small ones count), and the
+ * sum that the product is divided by is that of the rounded ones.
  * kv_max: the longest n_b expected (0: cache->rows); it decides how the keys are split over workgroups and never what is computed.
  * workspace: seedmi_kv_attention_workspace_bytes() bytes (may be 0), 256-byte aligned, initialised once after allocation by
  * seedmi_kv_attention_workspace_init (stream-ordered: its first 4 KiB are arrival counters, which every call leaves at zero again; the rest
- * may hold anything).  One workspace serves any calls whose bytes it covers, one after the other; calls that may overlap need one each. */
+ * may hold anything).  An initialisation that is recorded into a graph runs with the graph's replays and not before.  One workspace serves
+ * any calls whose bytes it covers, one after the other; calls that may overlap need one each. */
 size_t seedmi_kv_attention_workspace_bytes(const seedmi_kv_cache_t* cache, int B, int T, int H, int kv_max, int prefix_len);
 int seedmi_kv_attention_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
 int seedmi_kv_attention(const seedmi_kv_cache_t* cache, const seedmi_kv_cache_t* prefix, int prefix_len, const void* q, int ldq, void* out,
@@ -522,7 +524,8 @@ int seedmi_llama_decode_slots(const seedmi_llama_weights_t* w, const void* tok_i
  * prefix_len > 0 (a prompt that all slots share; prefix is a host array [layers] or NULL).  Positions are prefix_len + past + t.  past_max:
  * the longest past expected (host), for the position check and the split of the keys.  Everything else is seedmi_llama_forward: the same
  * GEMMs on the same workspace, T = 1 the decode path.  No launch argument depends on the lengths: a captured step replays as they grow.
- * attn_workspace: seedmi_kv_attention_workspace_bytes(&kv[0], batch, T, heads, past_max + T, prefix_len) bytes, initialised once. */
+ * attn_workspace: seedmi_kv_attention_workspace_bytes(&kv[0], batch, T, heads, past_max + T, prefix_len) bytes, initialised once.  Every
+ * layer's caches, the prefix and the workspaces are checked before the first launch: a refused call leaves the caches as they were. */
 int seedmi_llama_forward_kv(const seedmi_llama_weights_t* w, const seedmi_kv_cache_t* kv, const seedmi_kv_cache_t* prefix, int prefix_len,
                             const void* ids_i64, int batch, int T, const void* past_lens_i32, int past_max, int last_only, void* logits,
                             int ldl, void* attn_workspace, size_t attn_workspace_bytes, void* workspace, size_t workspace_bytes,

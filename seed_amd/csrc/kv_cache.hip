@@ -267,10 +267,9 @@ SEEDMI_DEVINL float add_pair(uint32_t w, float acc) {
 #endif
 }
 // Probabilities are rounded to the element for the product with the values, whose matrix instructions take operands of one type: in bf16 the
-// error against 64 bits is 0.0017 - 0.0019 relative, 0.0016 - 0.0018 of it the output's own rounding (fp16: 0.00022, 0.00021).
-// The sum of a row is that of its probabilities as they are rounded: out is then a mean of the values with
-// weights that add up to one, in every kernel.  (A sum of unrounded ones is off by what the roundings have in common: 387 equal scores of 400
-// made every output 0.92 half steps of the type too small.)
+// error against 64 bits is 0.0017 - 0.0019 relative, 0.0016 - 0.0018 of it the output's own rounding (fp16: 0.00022, 0.00021).  The sum of a
+// row is that of its probabilities as they are rounded: out is then a mean of the values with weights that add up to one, in every kernel.
+// (A sum of unrounded ones is off by what the roundings have in common: 387 equal scores of 400 made every output 0.92 half steps too small.)
 SEEDMI_DEVINL float add_probabilities(const uint4& w, float acc) { return add_pair(w.w, add_pair(w.z, add_pair(w.y, add_pair(w.x, acc)))); }
 
 // a product that is rounded before it is used (the compiler would be free to fuse it)
@@ -473,8 +472,9 @@ SEEDMI_DEVINL float2 load_pair(const float* p) {
     return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
 }
 // The last workgroup of a unit to get here joins the unit's rows, in the order of their parts whoever is last: no second launch.  Rows
-// first .. + n of the group that starts at token `base`, key head kvh; token row t of the group sees seen0 + t * seen_step keys (or none).  Every part's stores are past the L2s (waited for) before the
-// workgroup's arrival is counted; the counter wraps to zero with the last arrival.  Workgroups wait for nobody.
+// first .. + n of the group that starts at token `base`, key head kvh; token t of the group sees seen0 + t * seen_step keys (or none).  Every
+// part's stores are past the L2s (waited for) before the workgroup's arrival is counted; the counter wraps to zero with the last arrival.
+// Workgroups wait for nobody.
 template <int HD>
 SEEDMI_DEVINL void join_in_place(const AttnArgs& a, int unit, int base, int kvh, int first, int n, int seen0, int seen_step, float* lds) {
     constexpr int LPR = HD / 4, SLOTS = 256 / LPR, BATCH = 4;

@@ -2,8 +2,9 @@
 that all slots share (include/seedmi.h: seedmi_kv_append / seedmi_kv_read / seedmi_kv_attention).
 
 ``LlamaEngine`` keeps its static caches in 16 bits, one layout for all layers; these classes are the same caches for a serving loop of
-its own: ``KVCache.new`` holds 1.03 bytes a value in the 8-bit block format ("mx8": e4m3 with one power-of-two scale per 32 values, each
-value off by up to 2^-4 of itself, 2.7 % rms) or two in the 16-bit one ("16"), ``KVCache.wrap`` takes tensors that are there already (an engine's ``k_cache[i]`` / ``v_cache[i]`` among them).
+its own: ``KVCache.new`` holds 1.03 bytes a value in the 8-bit block format ("mx8": e4m3 with one power-of-two scale per 32 values; a value
+is off by up to 2^-4 of itself, the smallest of a block by more, 2.7 % rms) or two in the 16-bit one ("16"), ``KVCache.wrap`` takes tensors
+that are there already (an engine's ``k_cache[i]`` / ``v_cache[i]`` among them).
 A decode step is ``q = cache.append(qkv, cos, sin, lens, heads=H)`` and ``out = attention(q, lens + T)`` with an attention made once by
 ``KVAttention``; drafted chunks and prompt chunks are the same calls with more tokens per slot.
 
